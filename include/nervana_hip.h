@@ -231,6 +231,68 @@ int ng_pool_bprop(const ng_pool_params* p, int dtype, int op,
                   const void* I, const void* E, void* gradI, unsigned flags,
                   void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- block-scaled ("MX") matrices -----------------------------------------------
+ * No counterpart in the reference, whose narrowest storage is fp16 with stochastic
+ * rounding (nervanagpu/float_ew.py:182-201).  Blocks of 32 values along one axis
+ * share a power of two (OCP MXFP4 and MXINT8):
+ *   value = element * 2^(scale - 127); scale 255: every value of the block is NaN
+ *   NG_MX_FP4   0, 0.5, 1, 1.5, 2, 3, 4, 6 and a sign (4 bits)
+ *   NG_MX_INT8  code / 64, code -127 .. 127
+ * A line is one run of the blocked axis (`depth` values, nb = ceil(depth / 32)
+ * blocks).  codes: line after line, 16 (fp4) or 32 (int8) bytes a block, value 2i
+ * of a line in the low half of byte i; unused codes of the last block are zero.
+ * scales: a byte per block, lines of nb rounded up to a multiple of 8 bytes (what
+ * the padding bytes hold does not matter).  Both 16-byte aligned. */
+enum ng_mx_format { NG_MX_NONE = 0, NG_MX_FP4 = 1, NG_MX_INT8 = 2 };
+
+/* A (dtype NG_F16 or NG_F32) -> codes and scales.  Element (line, i) of A is
+ * A[line * lda + i] (along = 1: the blocks run along the contiguous axis) or
+ * A[i * lda + line] (along = 0).  Rounding is to the nearest, ties to the even
+ * code; with NG_FLAG_SR each value takes one of its two neighbours with the
+ * probability that makes it right on average (element line * depth + i of the stream
+ * (seed, rng_stream)).  A block that holds an infinity or a NaN becomes NaN. */
+int ng_mx_quantize(int format, int dtype, const void* A, long lda, int along, int lines, int depth,
+                   void* codes, void* scales, unsigned flags, unsigned seed, unsigned rng_stream, void* stream);
+/* out (dtype NG_F16 or NG_F32, laid out like A above) = the values, rounded to the
+ * nearest where fp16 does not hold them exactly */
+int ng_mx_dequantize(int format, const void* codes, const void* scales, int lines, int depth,
+                     int dtype, void* out, long ldo, int along, void* stream);
+
+/* Activation function of a (rows, cols) matrix with an 8-bit checkpoint of its
+ * input for the backward pass (NG_MX_INT8, a line per row).
+ *   ng_act_fprop  O = f(I); codes and scales, unless NULL, receive I
+ *   ng_act_bprop  gradI = E * f'(the values of the checkpoint); gradI may be E
+ * E, O and gradI have the dtype (NG_F16 or NG_F32) of I; ldi, ldo, lde, ldg are row
+ * pitches in elements. */
+enum ng_act { NG_ACT_RELU = 0, NG_ACT_SIG = 1, NG_ACT_TANH = 2, NG_ACT_SILU = 3, NG_ACT_GELU = 4 };
+int ng_act_fprop(int act, int dtype, int rows, int cols, const void* I, long ldi, void* O, long ldo,
+                 void* codes, void* scales, void* stream);
+int ng_act_bprop(int act, int dtype, int rows, int cols, const void* codes, const void* scales,
+                 const void* E, long lde, void* gradI, long ldg, void* stream);
+
+/* C = round(beta*C + relu(alpha * A.B)) where A (m, k) and B (k, n) are block
+ * scaled along k, or one of them is and the other is a dense fp16 matrix:
+ *   fp4 . fp4, fp4 . fp16, fp16 . fp4, int8 . fp16, fp16 . int8.
+ * C is fp16 or fp32 (c_dtype), row-major with row pitch ldc; fp32 accumulation.
+ * Block-scaled operand: format, codes, scales; lines are the rows of A / the columns
+ * of B.  Beside a dense operand its values are first rounded to fp16, which changes
+ * nothing if they came from fp16.
+ * Dense operand: format NG_MX_NONE, codes = the matrix, element (line, i) at
+ * [line * ld + i] (along = 1) or [i * ld + line] (along = 0).
+ * flags, seed, rng_stream and the order of operations are those of ng_gemm.
+ * workspace: 16-byte aligned, ng_mx_gemm_workspace_bytes() (0: may be NULL). */
+typedef struct ng_mx_operand {
+    int format;
+    int along;
+    long ld;
+    const void* codes;
+    const void* scales;
+} ng_mx_operand;
+int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const ng_mx_operand* B, void* C, int ldc,
+               float alpha, float beta, unsigned flags, unsigned seed, unsigned rng_stream,
+               void* workspace, size_t workspace_bytes, void* stream);
+size_t ng_mx_gemm_workspace_bytes(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const ng_mx_operand* B);
+
 /* ---- small data-movement helpers ---------------------------------------------
  * transpose / dimShuffle / fp32 convert kernels of nervanagpu/float_ew.py:1325-1428 */
 int ng_transpose(int dtype, const void* in, void* out, int rows, int cols, void* stream);

@@ -7,4 +7,5 @@ mirrors `from nervanagpu import NervanaGPU, GPUTensor` of the reference
 allocation; there is no CPU fallback.
 """
 from .nervanagpu import NervanaGPU, GPUTensor, OpTreeNode  # noqa: F401
+from .mx import MXTensor  # noqa: F401
 from ._lib import NervanaGPUError  # noqa: F401

@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(_HERE, "libnervana_hip.so")
 COMMON_HEADER = os.path.join(_HERE, "csrc", "ng_device_common.h")
 
 NG_F16, NG_F32, NG_U8, NG_I8 = 0, 1, 2, 3
+NG_MX_NONE, NG_MX_FP4, NG_MX_INT8 = 0, 1, 2
 FLAG_SR, FLAG_RELU = 1, 2
 
 
@@ -34,6 +35,10 @@ class PoolParams(ctypes.Structure):
     _fields_ = [(n, c_int) for n in (
         "N", "C", "D", "H", "W", "J", "T", "R", "S", "K", "M", "P", "Q",
         "pad_j", "pad_d", "pad_h", "pad_w", "str_j", "str_d", "str_h", "str_w")]
+
+
+class MxOperand(ctypes.Structure):
+    _fields_ = [("format", c_int), ("along", c_int), ("ld", c_long), ("codes", c_void_p), ("scales", c_void_p)]
 
 
 # name -> (restype, argtypes); every int-returning entry is status-checked
@@ -105,6 +110,16 @@ _SIGNATURES = {
     "ng_pool_workspace_bytes": (c_size_t, [POINTER(PoolParams), c_int, c_int]),
     "ng_pool_bprop": (c_int, [POINTER(PoolParams), c_int, c_int, c_void_p, c_void_p, c_void_p, c_uint,
                               c_void_p, c_size_t, c_void_p]),
+    "ng_mx_quantize": (c_int, [c_int, c_int, c_void_p, c_long, c_int, c_int, c_int, c_void_p, c_void_p,
+                               c_uint, c_uint, c_uint, c_void_p]),
+    "ng_mx_dequantize": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p, c_long, c_int, c_void_p]),
+    "ng_act_fprop": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p,
+                             c_void_p]),
+    "ng_act_bprop": (c_int, [c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_long, c_void_p, c_long,
+                             c_void_p]),
+    "ng_mx_gemm": (c_int, [c_int, c_int, c_int, c_int, POINTER(MxOperand), POINTER(MxOperand), c_void_p, c_int,
+                           c_float, c_float, c_uint, c_uint, c_uint, c_void_p, c_size_t, c_void_p]),
+    "ng_mx_gemm_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, POINTER(MxOperand), POINTER(MxOperand)]),
     "ng_transpose": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_void_p]),
     "ng_dimshuffle": (c_int, [c_int, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p]),
     "ng_fp32_convert": (c_int, [c_int, c_void_p, c_void_p, c_size_t, c_void_p]),

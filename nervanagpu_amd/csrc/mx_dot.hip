@@ -1,0 +1,240 @@
+// Products of block-scaled matrices: C = round(beta*C + relu(alpha * A.B)).
+#include "mx_gemm.h"
+
+#include <algorithm>
+
+namespace ng {
+
+// A dense operand as the kernels want it: lines of 16-byte chunks with the
+// contraction contiguous and zeros beyond it.  64 lines x 64 values through LDS.
+__global__ __launch_bounds__(256)
+void mx_pack_kernel(const unsigned short* __restrict__ X, long ld, int along, int lines, int depth, int padded,
+                    unsigned short* __restrict__ out)
+{
+    __shared__ unsigned short tile[64][66];
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+    const int line0 = (int)blockIdx.x * 64, i0 = (int)blockIdx.y * 64;
+#pragma unroll 4
+    for (int j = ty; j < 64; j += 4) {
+        const int line = line0 + (along ? j : tx), i = i0 + (along ? tx : j);
+        const unsigned short v = (line < lines && i < depth) ? X[along ? (long)line * ld + i : (long)i * ld + line] : (unsigned short)0;
+        tile[along ? j : tx][along ? tx : j] = v;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int j = ty; j < 64; j += 4)
+        if (line0 + j < lines && i0 + tx < padded) out[(long)(line0 + j) * padded + i0 + tx] = tile[j][tx];
+}
+
+struct MxArgs {
+    int c_dtype, m, n, k;
+    ng_mx_operand A, B;
+    void* C; int ldc;
+    float alpha, beta;
+    unsigned flags, seed, rng_stream;
+    char* ws; size_t ws_bytes;
+    hipStream_t stream;
+};
+
+static int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+static int padded_depth(int k) { return ceil_div(k, 8) * 8; }
+
+// a dense operand that the kernels can read where it lies
+static bool dense_in_place(const ng_mx_operand& o, int lines, int k)
+{
+    return o.along && ((uintptr_t)o.codes & 15) == 0 && k % 8 == 0 && (lines <= 1 || (o.ld % 8 == 0 && o.ld < (1L << 21)));
+}
+
+static size_t pack_bytes(const ng_mx_operand& o, int lines, int k)
+{
+    if (o.format != NG_MX_NONE || dense_in_place(o, lines, k)) return 0;
+    return align_up((size_t)lines * padded_depth(k) * 2, 256);
+}
+
+struct MxPlan { int bm, bn, bk, splits; };
+
+// as many slices of the contraction as give about one workgroup per CU, each at least
+// four tiles deep
+static int choose_slices(int out_tiles, int k_tiles, size_t slice_bytes, size_t ws_bytes)
+{
+    const int cus = device_cu_count();
+    int splits = std::max(1, cus / std::max(out_tiles, 1));
+    splits = std::min(splits, std::max(1, k_tiles / 4));
+    if (ws_bytes != SIZE_MAX && slice_bytes) splits = (int)std::min<size_t>((size_t)splits, std::max<size_t>(1, ws_bytes / slice_bytes));
+    while (splits > 1 && (splits - 1) * ceil_div(k_tiles, splits) >= k_tiles) splits--;
+    return std::max(splits, 1);
+}
+
+static bool is_44(const ng_mx_operand& A, const ng_mx_operand& B) { return A.format == NG_MX_FP4 && B.format == NG_MX_FP4; }
+
+static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_mx_operand& B, size_t ws_bytes)
+{
+    MxPlan p{128, 128, is_44(A, B) ? 128 : 64, 1};
+    const int tiles = ceil_div(m, p.bm) * ceil_div(n, p.bn);
+    p.splits = choose_slices(tiles, ceil_div(k, p.bk), (size_t)m * n * 4, ws_bytes);
+    return p;
+}
+
+static MxSide make_side(const ng_mx_operand& o, int lines, int k)
+{
+    MxSide s;
+    s.data = (const char*)o.codes;
+    s.scales = (const char*)o.scales;
+    s.lines = lines;
+    if (o.format == NG_MX_NONE) {
+        s.pitch = o.ld * 2;
+        s.scale_pitch = 0;
+        s.chunks = k / 8;
+        s.blocks = 0;
+    } else {
+        s.pitch = mx_code_pitch(o.format, k);
+        s.scale_pitch = mx_scale_pitch(k);
+        s.chunks = (int)(s.pitch / 16);
+        s.blocks = mx_blocks(k);
+    }
+    return s;
+}
+
+static unsigned mx_sr_bits(unsigned flags, int dtype)
+{
+    if (!(flags & NG_FLAG_SR)) return 0;
+    unsigned bits = flags >> 16;
+    if (bits == 0) bits = 10;
+    return std::max(1u, std::min(bits, dtype == NG_F16 ? 10u : 15u));
+}
+
+template <typename T, int FA, int FB, class Epi>
+static void launch_tiles(const MxArgs& g, const MxSide& a, const MxSide& b, const Epi& epi, const CoreShape& s, dim3 grid)
+{
+    if constexpr (FA == NG_MX_FP4 && FB == NG_MX_FP4)
+        hipLaunchKernelGGL((mx44_kernel<128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
+    else
+        hipLaunchKernelGGL((mxmix_kernel<FA, FB, 128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
+}
+
+template <typename T, int FA, int FB>
+static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
+{
+    MxPlan p = choose_plan(g.m, g.n, g.k, g.A, g.B, g.ws_bytes);
+    CoreShape s;
+    s.m = g.m;
+    s.n = g.n;
+    s.k_tiles = ceil_div(g.k, p.bk);
+    s.passes = 1;
+    s.splits = p.splits;
+    s.tiles_m = ceil_div(g.m, p.bm);
+    s.tiles_n = ceil_div(g.n, p.bn);
+    const int tiles = s.tiles_m * s.tiles_n;
+    const dim3 grid(grid_tiles(tiles, s.splits), grid_slices(tiles, s.splits), 1);
+    ScaleStoreEpilogue<T> epi{(T*)g.C, 0, g.ldc, g.m, g.n, g.alpha, g.beta, (g.flags & NG_FLAG_RELU) ? 1u : 0u,
+                              mx_sr_bits(g.flags, g.c_dtype), g.seed, g.rng_stream,
+                              (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u};
+    if (s.splits == 1) {
+        launch_tiles<T, FA, FB>(g, a, b, epi, s, grid);
+        NG_CHECK_LAUNCH("mx product");
+    } else {
+        PartialEpilogue pe{(float*)g.ws, g.m, g.n, 1, (g.n % 8 == 0) ? 1u : 0u};
+        launch_tiles<T, FA, FB>(g, a, b, pe, s, grid);
+        NG_CHECK_LAUNCH("mx product slices");
+        launch_splitk_reduce<T, ScaleStoreEpilogue<T>>((const float*)g.ws, s.splits, 1, g.m, g.n, epi, g.stream);
+        NG_CHECK_LAUNCH("mx product sum");
+    }
+    return 0;
+}
+
+template <typename T>
+static int dispatch(const MxArgs& g, const MxSide& a, const MxSide& b)
+{
+    const int fa = g.A.format, fb = g.B.format;
+    if (fa == NG_MX_FP4 && fb == NG_MX_FP4)   return launch_product<T, NG_MX_FP4, NG_MX_FP4>(g, a, b);
+    if (fa == NG_MX_FP4 && fb == NG_MX_NONE)  return launch_product<T, NG_MX_FP4, NG_MX_NONE>(g, a, b);
+    if (fa == NG_MX_NONE && fb == NG_MX_FP4)  return launch_product<T, NG_MX_NONE, NG_MX_FP4>(g, a, b);
+    if (fa == NG_MX_INT8 && fb == NG_MX_NONE) return launch_product<T, NG_MX_INT8, NG_MX_NONE>(g, a, b);
+    return launch_product<T, NG_MX_NONE, NG_MX_INT8>(g, a, b);
+}
+
+static int check_operand(const char* name, const ng_mx_operand* o, int lines, int k)
+{
+    if (!o) return fail(-90, "ng_mx_gemm: null operand %s", name);
+    if (o->format < NG_MX_NONE || o->format > NG_MX_INT8) return fail(-91, "ng_mx_gemm: unknown format %d of %s", o->format, name);
+    if (!lines || !k) return 0;
+    if (!o->codes || (o->format != NG_MX_NONE && !o->scales)) return fail(-92, "ng_mx_gemm: null operand %s", name);
+    if (o->format != NG_MX_NONE && ((((uintptr_t)o->codes) | ((uintptr_t)o->scales)) & 15))
+        return fail(-93, "ng_mx_gemm: codes and scales of %s must be 16-byte aligned", name);
+    if (o->format == NG_MX_NONE && o->ld < (o->along ? k : lines) && (o->along ? lines : k) > 1)
+        return fail(-94, "ng_mx_gemm: leading dimension of %s smaller than row length", name);
+    return 0;
+}
+
+// formats, extents and what the kernels' 32-bit offsets hold; 0 or a status
+static int check_product(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const ng_mx_operand* B)
+{
+    if (c_dtype != NG_F16 && c_dtype != NG_F32) return fail(-95, "ng_mx_gemm: C must be fp16 or fp32");
+    if (m < 0 || n < 0 || k < 0) return fail(-96, "ng_mx_gemm: negative extent");
+    int rc = check_operand("A", A, m, k);
+    if (!rc) rc = check_operand("B", B, n, k);
+    if (rc) return rc;
+    const bool ok = (A->format == NG_MX_FP4 && B->format == NG_MX_FP4) || ((A->format == NG_MX_NONE) != (B->format == NG_MX_NONE));
+    if (!ok) return fail(-97, "ng_mx_gemm: formats %d and %d do not multiply (fp4 by fp4, or one dense fp16 operand)", A->format, B->format);
+    if (k >= (1 << 21)) return fail(-98, "ng_mx_gemm: contraction of 2^21 or more");
+    if ((long)m * n >= (1L << 32)) return fail(-99, "ng_mx_gemm: output of 2^32 or more elements");
+    return 0;
+}
+
+}  // namespace ng
+
+using namespace ng;
+
+extern "C" {
+
+size_t ng_mx_gemm_workspace_bytes(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const ng_mx_operand* B)
+{
+    if (!A || !B || m <= 0 || n <= 0 || k <= 0) return 0;
+    (void)c_dtype;
+    const MxPlan p = choose_plan(m, n, k, *A, *B, SIZE_MAX);
+    const size_t slices = p.splits > 1 ? align_up((size_t)p.splits * m * n * 4, 256) : 0;
+    return slices + pack_bytes(*A, m, k) + pack_bytes(*B, n, k);
+}
+
+int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const ng_mx_operand* B, void* C, int ldc,
+               float alpha, float beta, unsigned flags, unsigned seed, unsigned rng_stream,
+               void* workspace, size_t workspace_bytes, void* stream)
+{
+    int rc = check_product(c_dtype, m, n, k, A, B);
+    if (rc) return rc;
+    if (!m || !n) return 0;
+    if (!C) return fail(-100, "ng_mx_gemm: null C");
+    if (ldc < n && m > 1) return fail(-101, "ng_mx_gemm: leading dimension of C smaller than row length");
+    const size_t need = ng_mx_gemm_workspace_bytes(c_dtype, m, n, k, A, B);
+    if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
+        return fail(-102, "ng_mx_gemm: this product needs %zu bytes of 16-byte aligned workspace, got %zu", need,
+                    workspace ? workspace_bytes : (size_t)0);
+    MxArgs g{c_dtype, m, n, k, *A, *B, C, ldc, alpha, beta, flags, seed, rng_stream,
+             (char*)workspace, workspace_bytes, (hipStream_t)stream};
+    // dense operands that are not laid out for the kernels are copied behind the slices
+    char* end = g.ws + need;
+    int lines = m;
+    for (ng_mx_operand* o : {&g.A, &g.B}) {
+        const size_t bytes = pack_bytes(*o, lines, k);
+        if (bytes && k) {
+            end -= bytes;
+            const int padded = padded_depth(k);
+            if (ceil_div(k, 64) > 65535) return fail(-98, "ng_mx_gemm: contraction too long");
+            hipLaunchKernelGGL(mx_pack_kernel, dim3((unsigned)ceil_div(lines, 64), (unsigned)ceil_div(padded, 64)), dim3(256), 0,
+                               g.stream, (const unsigned short*)o->codes, o->ld, o->along, lines, k, padded, (unsigned short*)end);
+            NG_CHECK_LAUNCH("mx pack");
+            o->codes = end;
+            o->along = 1;
+            o->ld = padded;
+        }
+        lines = n;
+    }
+    g.ws_bytes = (size_t)(end - g.ws);
+    const int kd = (g.A.format == NG_MX_NONE || g.B.format == NG_MX_NONE) ? padded_depth(k) : k;
+    const MxSide a = make_side(g.A, m, g.A.format == NG_MX_NONE ? kd : k);
+    const MxSide b = make_side(g.B, n, g.B.format == NG_MX_NONE ? kd : k);
+    return c_dtype == NG_F16 ? dispatch<_Float16>(g, a, b) : dispatch<float>(g, a, b);
+}
+
+}  // extern "C"

@@ -16,12 +16,16 @@ from ctypes import c_void_p
 import numpy as np
 
 from . import _lib
+from .mx import MXTensor
 from .float_ew import call_compensated_sum, call_compound_kernel
 
 _none_slice = slice(None, None, None)
 
 _DTYPE_CODE = {np.dtype(np.float16): _lib.NG_F16, np.dtype(np.float32): _lib.NG_F32,
                np.dtype(np.uint8): _lib.NG_U8, np.dtype(np.int8): _lib.NG_I8}
+
+
+_ACT_CODE = {"relu": 0, "sig": 1, "tanh": 2, "silu": 3, "gelu": 4}
 
 
 def _contiguous_strides(shape):
@@ -679,6 +683,166 @@ class NervanaGPU(object):
         assert k == B.shape[0]
 
         return self._gemm(A, B, C, m, n, k, lda, ldb, ldc, alpha, beta, relu, repeat, 1, 0, 0, 0, 1)
+
+    # ---- block-scaled matrices and 8-bit checkpoints (not in the reference) -------------
+
+    def mx_empty(self, shape, fmt="fp4", axis=1, name=None, rounding=None):
+        """allocate a block-scaled matrix (see mx.MXTensor); rounding: stochastic
+        when true, default as this backend stores its other tensors"""
+        return MXTensor(self, shape, fmt, axis, name=name, rounding=self.round_mode if rounding is None else rounding)
+
+    def mx_array(self, ary, fmt="fp4", axis=1, name=None, rounding=None):
+        """a host matrix converted to a block-scaled one"""
+        return self.mx_empty(ary.shape, fmt, axis, name, rounding).set(ary)
+
+    def _mx_dense(self, A, axis, what):
+        """(pitch, whether lines along `axis` are contiguous) of a dense 2-D tensor"""
+        assert isinstance(A, GPUTensor) and len(A.shape) == 2 and not A.take_array, "%s must be a 2-D tensor" % what
+        if not A.size:
+            return A.shape[axis], 1
+        assert min(A.strides) >= 1 and (1 in A.strides), "one dimension of %s must be contiguous" % what
+        if A.strides[axis] == 1 and (A.strides[1 - axis] >= A.shape[axis] or A.shape[1 - axis] <= 1):
+            return A.strides[1 - axis], 1
+        assert A.strides[1 - axis] == 1, "one dimension of %s must be contiguous" % what
+        return A.strides[axis], 0
+
+    def mx_quantize(self, A, out, repeat=1):
+        """out = A in blocks of 32 values that share a power of two.  A: fp16 or fp32
+        matrix with one contiguous dimension.  Rounds to the nearest code (ties to
+        even), or stochastically if out.rounding is set: then every value is right on
+        average.  A block with an infinity or a NaN becomes NaN.  Returns out."""
+        assert isinstance(out, MXTensor) and A.shape == out.shape
+        if A.dtype.type not in (np.float16, np.float32):
+            raise TypeError("Only floating point tensors can be quantized.")
+        ld, along = self._mx_dense(A, out.axis, "A")
+        if not out.size:
+            return out
+        for r in range(repeat):
+            flags, (seed, sid) = (_lib.FLAG_SR, self._next_rng_stream()) if out.rounding else (0, (0, 0))
+            _lib.call("ng_mx_quantize", out.fmt_code, _DTYPE_CODE[A.dtype], A.ptr, ld, along, out.lines, out.depth,
+                      out.codes.ptr, out.scales.ptr, flags, seed, sid, self.stream)
+        return out
+
+    def mx_dequantize(self, A, out):
+        """out (fp16 or fp32) = the values of the block-scaled A; returns out"""
+        assert isinstance(A, MXTensor) and A.shape == out.shape
+        if out.dtype.type not in (np.float16, np.float32):
+            raise TypeError("Only floating point tensors can be dequantized into.")
+        ld, along = self._mx_dense(out, A.axis, "out")
+        if A.size:
+            _lib.call("ng_mx_dequantize", A.fmt_code, A.codes.ptr, A.scales.ptr, A.lines, A.depth, _DTYPE_CODE[out.dtype],
+                      out.ptr, ld, along, self.stream)
+        return out
+
+    def _mx_side(self, X, axis, what):
+        """an operand of mx_dot whose contraction is its axis `axis`"""
+        if isinstance(X, MXTensor):
+            if X.axis != axis:
+                raise ValueError("the blocks of %s must run along the contraction (axis %d)" % (what, axis))
+            return X.operand()
+        assert X.dtype.type is np.float16, "a dense operand of mx_dot must be fp16"
+        ld, along = self._mx_dense(X, axis, what)
+        return _lib.MxOperand(_lib.NG_MX_NONE, along, ld, X.ptr if X.size else None, None)
+
+    def mx_dot(self, A, B, C, alpha=1.0, beta=0.0, relu=False, repeat=1):
+        """
+        C = relu(alpha * A * B) + beta * C for block-scaled operands
+
+        A (m, k), B (k, n): both fp4, or one of them fp4 or int8 and the other a dense
+        fp16 tensor (any order of its axes; the values of the block-scaled one are then
+        taken as fp16).  Blocks run along k: A has axis 1, B has axis 0.
+        C: fp16 or fp32, rows or columns contiguous; stochastic rounding as in dot.
+        """
+        if not isinstance(A, MXTensor) and not isinstance(B, MXTensor):
+            raise TypeError("mx_dot needs a block-scaled operand (dot multiplies dense ones)")
+        if isinstance(A, MXTensor) and isinstance(B, MXTensor) and (A.fmt, B.fmt) != ("fp4", "fp4"):
+            raise TypeError("block-scaled operands must both be fp4, or one operand a dense fp16 tensor")
+        if C.dtype.type not in (np.float16, np.float32):
+            raise TypeError("Only floating point dot currently supported.")
+        (m, k), n = A.shape, B.shape[1]
+        assert C.shape == (m, n) and B.shape[0] == k
+        assert len(C.strides) == 2 and not C.take_array
+        a, b = self._mx_side(A, 1, "A"), self._mx_side(B, 0, "B")
+        ldc, by_rows = self._mx_dense(C, 1, "C")
+        if not by_rows:
+            # columns contiguous: the transposed product
+            m, n, a, b = n, m, b, a
+        code = _DTYPE_CODE[C.dtype]
+        flags = 0
+        if C.rounding:
+            flags |= 1 | (int(C.rounding) << 16)
+        if relu:
+            flags |= 2
+        if not C.size:
+            return C
+        need = _lib.load().ng_mx_gemm_workspace_bytes(code, m, n, k, a, b)
+        ws, ws_bytes = self._get_scratch(need)
+        stream = self.stream
+
+        def launch():
+            seed, sid = self._next_rng_stream() if C.rounding else (0, 0)
+            _lib.call("ng_mx_gemm", code, m, n, k, a, b, C.ptr, ldc, alpha, beta, flags, seed, sid, int(ws), ws_bytes, stream)
+
+        if repeat > 1:
+            for r in range(max(repeat // 10, 1)):
+                launch()
+        if self.bench or repeat > 1:
+            start, end = self._get_events()
+            start.record(stream)
+        for r in range(repeat):
+            launch()
+        if self.bench or repeat > 1:
+            end.record(stream)
+            end.synchronize()
+            msecs = end.time_since(start) / repeat
+            gflops = (m * n * k * 2.0) / (msecs * 1000000.0)
+            print("%7.3f msecs %4.0f gflops (mx_dot: %d,%d,%d)" % (msecs, gflops, m, n, k))
+            if repeat > 1:
+                return gflops
+        return C
+
+    def _act_operand(self, X, like, what):
+        """row pitch of an operand of an activation function"""
+        if X.dtype.type not in (np.float16, np.float32):
+            raise TypeError("Only floating point activations are supported.")
+        assert X.shape == like.shape and X.dtype == like.dtype, "%s must match the other operands" % what
+        ld, along = self._mx_dense(X, 1, what)
+        assert along, "rows of %s must be contiguous" % what
+        return ld
+
+    def _act_saved(self, saved, shape):
+        assert isinstance(saved, MXTensor) and saved.shape == tuple(shape)
+        if saved.fmt != "int8" or saved.axis != 1 or saved.rounding:
+            raise ValueError("a checkpoint of activations is an int8 MXTensor with axis 1 and nearest rounding")
+
+    def fprop_act(self, op, I, O, saved=None):
+        """
+        O = op(I), and saved (an MXTensor, fmt "int8", axis 1) = I, in one pass.
+
+        op: "relu", "sig", "tanh", "silu" (x sig(x)) or "gelu" (x times the normal
+        distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous
+        """
+        if op not in _ACT_CODE:
+            raise ValueError("unknown activation function %r (%s)" % (op, ", ".join(sorted(_ACT_CODE))))
+        ldi, ldo = self._act_operand(I, I, "I"), self._act_operand(O, I, "O")
+        if saved is not None:
+            self._act_saved(saved, I.shape)
+        if I.size:
+            _lib.call("ng_act_fprop", _ACT_CODE[op], _DTYPE_CODE[I.dtype], I.shape[0], I.shape[1], I.ptr, ldi, O.ptr, ldo,
+                      saved.codes.ptr if saved is not None else None, saved.scales.ptr if saved is not None else None, self.stream)
+        return O
+
+    def bprop_act(self, op, saved, E, grad_I):
+        """grad_I = E * op'(saved): the derivative is taken at the values the 8-bit
+        checkpoint of fprop_act stands for.  grad_I may be E."""
+        if op not in _ACT_CODE:
+            raise ValueError("unknown activation function %r (%s)" % (op, ", ".join(sorted(_ACT_CODE))))
+        lde, ldg = self._act_operand(E, E, "E"), self._act_operand(grad_I, E, "grad_I")
+        self._act_saved(saved, E.shape)
+        if E.size:
+            _lib.call("ng_act_bprop", _ACT_CODE[op], _DTYPE_CODE[E.dtype], E.shape[0], E.shape[1], saved.codes.ptr,
+                      saved.scales.ptr, E.ptr, lde, grad_I.ptr, ldg, self.stream)
+        return grad_I
 
     def compensated_sum(self, sum_tensor, cmp_tensor, add_tensor, cmp_scale=1.0, add_scale=1.0):
         """Kahan-compensated low-precision accumulate

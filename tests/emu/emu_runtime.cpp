@@ -22,7 +22,7 @@ namespace {
 
 constexpr size_t STACK_BYTES = 256 * 1024;
 
-struct PendingLoad { char* dst; bool is_dma; bool zero; unsigned char data[16]; };
+struct PendingLoad { char* dst; bool is_dma; bool zero; unsigned bytes; unsigned char data[16]; };
 
 struct Wave {
     int live = 0;                 // lanes that have not returned
@@ -57,8 +57,8 @@ void yield() { swapcontext(&g_cur->ctx, &g_main); }
 void apply(const PendingLoad& p)
 {
     if (!p.is_dma) return;
-    if (p.zero) std::memset(p.dst, 0, 16);
-    else std::memcpy(p.dst, p.data, 16);
+    if (p.zero) std::memset(p.dst, 0, p.bytes);
+    else std::memcpy(p.dst, p.data, p.bytes);
 }
 
 void fiber_entry()
@@ -103,11 +103,13 @@ void wave_exchange_sync()
     g_progress++;
 }
 
-void vmem_issue(char* lds_dst, const void* src16)
+void vmem_issue(char* lds_dst, const void* src16) { vmem_issue_bytes(lds_dst, src16, 16); }
+
+void vmem_issue_bytes(char* lds_dst, const void* src, unsigned bytes)
 {
     PendingLoad p;
-    p.dst = lds_dst; p.is_dma = true; p.zero = src16 == nullptr;
-    if (src16) std::memcpy(p.data, src16, 16);
+    p.dst = lds_dst; p.is_dma = true; p.zero = src == nullptr; p.bytes = bytes;
+    if (src) std::memcpy(p.data, src, bytes);
     if (g_late_loads) g_cur->vmem.push_back(p);
     else { apply(p); p.is_dma = false; g_cur->vmem.push_back(p); }
 }

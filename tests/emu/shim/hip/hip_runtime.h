@@ -76,6 +76,7 @@ void launch(dim3 grid, dim3 block, const std::function<void()>& body, const char
 
 // vector-memory operations of the current wavefront that s_waitcnt vmcnt counts
 void vmem_issue(char* lds_dst, const void* src16);   // 16 bytes to LDS (src16 == nullptr: zeros)
+void vmem_issue_bytes(char* lds_dst, const void* src, unsigned bytes);   // the same with 4 or 16 bytes
 void vmem_issue_plain();                             // a load into registers or a store
 void vmem_wait(int outstanding);
 
@@ -234,6 +235,16 @@ inline void buffer_load_chunk_to_lds(emu_rsrc_t rsrc, char* lds_base, unsigned b
     }
     emu::vmem_issue(lds_base + 16 * emu::cur->lane, src);
 }
+// the same with 4 bytes per lane: lane l writes lds_base + 4 l
+inline void buffer_load_dword_to_lds(emu_rsrc_t rsrc, char* lds_base, unsigned byte_offset)
+{
+    const char* src = nullptr;
+    if (emu_in_range(rsrc, (int)byte_offset, 0, 4)) {
+        src = rsrc.base + byte_offset;
+        emu_check_access(src, 4, "buffer load to LDS (4 bytes)");
+    }
+    emu::vmem_issue_bytes(lds_base + 4 * emu::cur->lane, src, 4);
+}
 }  // namespace ng
 
 // ---- wavefront-wide LDS read and matrix instructions ----------------------------------------
@@ -300,6 +311,88 @@ inline emu_float16_t __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float b, emu_
             sum += av * bv;
         }
         c[v] += sum;
+    }
+    return c;
+}
+
+// ---- lane permutes, byte permutes ----------------------------------------------------------
+// quad permutes only (control below 256): lane 4q + i reads lane 4q + (control >> 2i & 3)
+inline int __builtin_amdgcn_update_dpp(int, int v, int control, int, int, bool)
+{
+    char* slots = emu::wave_exchange_begin();
+    std::memcpy(slots + 64 * emu::cur->lane, &v, 4);
+    emu::wave_exchange_sync();
+    const int lane = emu::cur->lane;
+    int r;
+    std::memcpy(&r, slots + 64 * ((lane & ~3) + ((control >> (2 * (lane & 3))) & 3)), 4);
+    return r;
+}
+// bytes 0-3 of the selector's index space are those of `lo`, 4-7 those of `hi`
+inline unsigned __builtin_amdgcn_perm(unsigned hi, unsigned lo, unsigned selector)
+{
+    const unsigned long both = ((unsigned long)hi << 32) | lo;
+    unsigned r = 0;
+    for (int i = 0; i < 4; i++) r |= (unsigned)((both >> (8 * ((selector >> (8 * i)) & 7))) & 255) << (8 * i);
+    return r;
+}
+
+// ---- 4-bit floating point: sign, two exponent bits, one mantissa bit -------------------------
+inline float emu_fp4_value(unsigned code)
+{
+    static const float grid[8] = {0.0f, 0.5f, 1.0f, 1.5f, 2.0f, 3.0f, 4.0f, 6.0f};
+    return (code & 8) ? -grid[code & 7] : grid[code & 7];
+}
+// nearest, ties to the even code, saturating; the scale divides
+inline unsigned emu_fp4_code(float v, float scale)
+{
+    const float a = std::fabs(v) / scale;
+    const float unit = a < 2 ? 0.5f : a < 4 ? 1.0f : 2.0f;
+    unsigned code = 7;
+    if (a < 8) code = (unsigned)std::nearbyint(a / unit) + (a < 2 ? 0 : a < 4 ? 2 : 4);
+    if (code > 7) code = 7;
+    return code | (std::signbit(v) ? 8u : 0u);
+}
+inline unsigned __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(unsigned old, float a, float b, float scale, int byte)
+{
+    const unsigned v = emu_fp4_code(a, scale) | (emu_fp4_code(b, scale) << 4);
+    return (old & ~(255u << (8 * byte))) | (v << (8 * byte));
+}
+inline emu_half2_t __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(unsigned w, float scale, int byte)
+{
+    const unsigned v = (w >> (8 * byte)) & 255u;
+    emu_half2_t r = {(_Float16)(emu_fp4_value(v & 15) * scale), (_Float16)(emu_fp4_value(v >> 4) * scale)};
+    return r;
+}
+inline float emu_e8m0(int byte) { return byte == 255 ? NAN : std::ldexp(1.0f, byte - 127); }
+typedef int emu_int8v_t __attribute__((ext_vector_type(8)));
+// D = A (32 x 64) . B (64 x 32) + C of 4-bit operands (formats 4): lane l holds contraction values
+// 32 (l >> 5) .. + 31 of row / column l & 31 in its first four registers, low half of a byte first, and
+// byte `opsel` of its scale register scales them
+inline emu_float16_t __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(emu_int8v_t a, emu_int8v_t b, emu_float16_t c, int fa, int fb,
+                                                                     int opsel_a, int scale_a, int opsel_b, int scale_b)
+{
+    if (fa != 4 || fb != 4) std::abort();
+    char* slots = emu::wave_exchange_begin();
+    char* mine = slots + 64 * emu::cur->lane;
+    std::memcpy(mine, &a, 16);
+    std::memcpy(mine + 16, &b, 16);
+    const unsigned char sa = (unsigned char)(scale_a >> (8 * opsel_a)), sb = (unsigned char)(scale_b >> (8 * opsel_b));
+    mine[32] = (char)sa;
+    mine[33] = (char)sb;
+    emu::wave_exchange_sync();
+    const int lane = emu::cur->lane, col = lane & 31;
+    for (int v = 0; v < 16; v++) {
+        const int row = 8 * (v / 4) + 4 * (lane >> 5) + (v & 3);
+        double sum = 0.0;
+        for (int h = 0; h < 2; h++) {
+            const unsigned char* pa = (const unsigned char*)slots + 64 * (row + 32 * h);
+            const unsigned char* pb = (const unsigned char*)slots + 64 * (col + 32 * h) + 16;
+            float part = 0.0f;      // 32 products of small multiples of 1/4: exact
+            for (int k = 0; k < 32; k++)
+                part += emu_fp4_value((pa[k / 2] >> (4 * (k & 1))) & 15) * emu_fp4_value((pb[k / 2] >> (4 * (k & 1))) & 15);
+            sum += (double)part * emu_e8m0(pa[32]) * emu_e8m0(pb[17]);
+        }
+        c[v] = (float)(c[v] + sum);
     }
     return c;
 }
