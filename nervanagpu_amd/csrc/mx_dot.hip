@@ -55,12 +55,12 @@ static size_t pack_bytes(const ng_mx_operand& o, int lines, int k)
 struct MxPlan { int bm, bn, bk, splits; };
 
 // as many slices of the contraction as give about one workgroup per CU, each at least
-// four tiles deep
-static int choose_slices(int out_tiles, int k_tiles, size_t slice_bytes, size_t ws_bytes)
+// `least` tiles deep
+static int choose_slices(int out_tiles, int k_tiles, int least, size_t slice_bytes, size_t ws_bytes)
 {
     const int cus = device_cu_count();
     int splits = std::max(1, cus / std::max(out_tiles, 1));
-    splits = std::min(splits, std::max(1, k_tiles / 4));
+    splits = std::min(splits, std::max(1, k_tiles / least));
     if (ws_bytes != SIZE_MAX && slice_bytes) splits = (int)std::min<size_t>((size_t)splits, std::max<size_t>(1, ws_bytes / slice_bytes));
     while (splits > 1 && (splits - 1) * ceil_div(k_tiles, splits) >= k_tiles) splits--;
     return std::max(splits, 1);
@@ -70,9 +70,20 @@ static bool is_44(const ng_mx_operand& A, const ng_mx_operand& B) { return A.for
 
 static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_mx_operand& B, size_t ws_bytes)
 {
-    MxPlan p{128, 128, is_44(A, B) ? 128 : 64, 1};
-    const int tiles = ceil_div(m, p.bm) * ceil_div(n, p.bn);
-    p.splits = choose_slices(tiles, ceil_div(k, p.bk), (size_t)m * n * 4, ws_bytes);
+    const int cus = device_cu_count();
+    auto tiles = [&](int bm, int bn) { return (long)ceil_div(m, bm) * ceil_div(n, bn); };
+    MxPlan p{128, 128, 64, 1};
+    int least = 4;
+    if (is_44(A, B)) {
+        p.bk = 256;
+        least = 2;
+        if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2) p.bm = p.bn = 256;
+        else if (tiles(128, 128) <= cus / 2) p.bm = p.bn = 64;
+    } else if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2) {
+        p.bm = p.bn = 256;
+    }
+    const int out_tiles = (int)std::min<long>(tiles(p.bm, p.bn), 1 << 30);
+    p.splits = choose_slices(out_tiles, ceil_div(k, p.bk), least, (size_t)m * n * 4, ws_bytes);
     return p;
 }
 
@@ -105,18 +116,26 @@ static unsigned mx_sr_bits(unsigned flags, int dtype)
 }
 
 template <typename T, int FA, int FB, class Epi>
-static void launch_tiles(const MxArgs& g, const MxSide& a, const MxSide& b, const Epi& epi, const CoreShape& s, dim3 grid)
+static void launch_tiles(const MxArgs& g, const MxPlan& p, const MxSide& a, const MxSide& b, const Epi& epi, const CoreShape& s,
+                         dim3 grid)
 {
-    if constexpr (FA == NG_MX_FP4 && FB == NG_MX_FP4)
-        hipLaunchKernelGGL((mx44_kernel<128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
-    else
-        hipLaunchKernelGGL((mxmix_kernel<FA, FB, 128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
+    if constexpr (FA == NG_MX_FP4 && FB == NG_MX_FP4) {
+        if (p.bm == 256)      hipLaunchKernelGGL((mx44_kernel<256, 256, 256, 2, 4, 2, Epi>), grid, dim3(512), 0, g.stream, a, b, epi, s);
+        else if (p.bm == 128) hipLaunchKernelGGL((mx44_kernel<128, 128, 256, 2, 2, 2, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
+        else                  hipLaunchKernelGGL((mx44_kernel<64, 64, 256, 2, 2, 2, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
+    } else {
+        constexpr bool X_IS_A = FA != NG_MX_NONE;
+        constexpr int FMT = X_IS_A ? FA : FB;
+        const MxSide &x = X_IS_A ? a : b, &d = X_IS_A ? b : a;
+        if (p.bm == 256) hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 256, 256, 4, 2, 3, Epi>), grid, dim3(512), 0, g.stream, x, d, epi, s);
+        else             hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, x, d, epi, s);
+    }
 }
 
 template <typename T, int FA, int FB>
 static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
 {
-    MxPlan p = choose_plan(g.m, g.n, g.k, g.A, g.B, g.ws_bytes);
+    const MxPlan p = choose_plan(g.m, g.n, g.k, g.A, g.B, g.ws_bytes);
     CoreShape s;
     s.m = g.m;
     s.n = g.n;
@@ -131,11 +150,11 @@ static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
                               mx_sr_bits(g.flags, g.c_dtype), g.seed, g.rng_stream,
                               (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u};
     if (s.splits == 1) {
-        launch_tiles<T, FA, FB>(g, a, b, epi, s, grid);
+        launch_tiles<T, FA, FB>(g, p, a, b, epi, s, grid);
         NG_CHECK_LAUNCH("mx product");
     } else {
         PartialEpilogue pe{(float*)g.ws, g.m, g.n, 1, (g.n % 8 == 0) ? 1u : 0u};
-        launch_tiles<T, FA, FB>(g, a, b, pe, s, grid);
+        launch_tiles<T, FA, FB>(g, p, a, b, pe, s, grid);
         NG_CHECK_LAUNCH("mx product slices");
         launch_splitk_reduce<T, ScaleStoreEpilogue<T>>((const float*)g.ws, s.splits, 1, g.m, g.n, epi, g.stream);
         NG_CHECK_LAUNCH("mx product sum");

@@ -64,47 +64,45 @@ struct MxTile {
     static __device__ __forceinline__ int offset(int line, int c) { return line * LINE_BYTES + ((c ^ swizzle(line)) * 16); }
 };
 
-// Fetches one operand's tiles.  Addresses: a 64-bit base that steps along the
-// contraction plus 32-bit offsets inside the rows of the tile.
-template <class Tile, int ROWS, int NT, bool SCALES>
+// Fetches one operand's tiles: request i of a tile brings lines i * STEP .. of it.  The
+// swizzle repeats after STEP lines, so the requests differ by a scalar base alone and a
+// lane keeps one offset.  What does not exist reads as zero: lines behind the last one
+// lie behind the descriptor's end, chunks behind a line's last take an offset that does.
+template <class Tile, int NT>
 struct MxFetch {
-    static constexpr int DATA = Tile::CHUNKS / NT;
-    static_assert(Tile::CHUNKS % NT == 0, "tile chunks must divide evenly over threads");
-    unsigned off[DATA];
-    int col[DATA];
-    const char* base;
-    int left;                // chunks of a line not yet fetched
+    static constexpr int DATA = Tile::CHUNKS / NT, STEP = NT / Tile::CPR;
+    static_assert(Tile::CHUNKS % NT == 0 && NT % Tile::CPR == 0, "tile chunks must divide evenly over threads");
+    static_assert(DATA == 1 || (STEP / Tile::LP) % Tile::CPR == 0, "requests must be whole periods of the swizzle");
+    const char* base;        // of the next tile
+    int bytes;               // from there to the end of the operand, 2^31 - 1 if that is further
+    int pitch;
+    unsigned off;
+    int col, left;           // the lane's chunk of a line, chunks of a line not yet fetched
     __device__ __forceinline__ void init(const MxSide& s, int row0, int kt, int tid)
     {
+        pitch = (int)s.pitch;
         base = s.data + (long)row0 * s.pitch + (long)kt * (Tile::CPR * 16);
+        // a tile's lines span less than 2^30 bytes and so does a line, so a clamped end stays out of reach
+        bytes = (int)min((long)(s.lines - 1 - row0) * s.pitch + (long)s.chunks * 16 - (long)kt * (Tile::CPR * 16), 0x7FFFFFFFl);
         left = s.chunks - kt * Tile::CPR;
-#pragma unroll
-        for (int i = 0; i < DATA; i++) {
-            int line;
-            Tile::chunk_pos(tid + i * NT, line, col[i]);
-            off[i] = row0 + line < s.lines ? (unsigned)line * (unsigned)s.pitch + (unsigned)col[i] * 16u : NG_OOB_OFFSET;
-        }
+        int line;
+        Tile::chunk_pos(tid, line, col);
+        off = (unsigned)line * (unsigned)s.pitch + (unsigned)col * 16u;
     }
-    __device__ __forceinline__ void issue(int i, char* lds, int wave) const
+    __device__ __forceinline__ unsigned lane_offset() const { return col < left ? off : NG_OOB_OFFSET; }
+    __device__ __forceinline__ void issue(int i, unsigned lane_off, char* lds, int wave) const
     {
-        buffer_load_chunk_to_lds(make_rsrc(base), lds + (i * NT + wave * 64) * 16, col[i] < left ? off[i] : NG_OOB_OFFSET);
+        const int skip = i * STEP * pitch;
+        const BufferRsrc r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + skip), 0, max(bytes - skip, 0), 0x00020000);
+        buffer_load_chunk_to_lds(r, lds + (i * NT + wave * 64) * 16, lane_off);
     }
     __device__ __forceinline__ void advance()
     {
         base += Tile::CPR * 16;
+        bytes -= Tile::CPR * 16;
         left -= Tile::CPR;
     }
 };
-
-// fp16 values 8 s .. 8 s + 7 of a lane's 32-value fp4 block
-__device__ __forceinline__ half8_t mx_expand_fp4(unsigned w, float scale)
-{
-    const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 0);
-    const half2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 1);
-    const half2_t c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 2);
-    const half2_t d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w, scale, 3);
-    return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
-}
 
 // Scale of an int8 block as fp16 factors.  code * 2^e is formed as
 // ((1024 + code + 128) * s1 - 1152 * s1) * s2 with s1 s2 = 2^e: the bytes become
@@ -143,52 +141,68 @@ __device__ __forceinline__ unsigned mx_scale_mask(int blocks, int first)
     return valid >= 4 ? 0xFFFFFFFFu : valid <= 0 ? 0u : (1u << (8 * valid)) - 1u;
 }
 
-// Scale dwords of a tile: 64 lines per wavefront request, the requests of both
-// operands dealt to the wavefronts in turn; every wavefront issues the same number.
+// Scales of the fp4 . fp4 kernel.  Fetched a dword (a tile of 128 values) per line they
+// would be as many memory requests as the codes, since every line is a request of its own.
+// So four lanes take the four dwords of one line (four tiles, a group) and a request
+// serves 16 lines of them.  A tile's turn fetches a quarter of the group after next
+// into a ring of three, so every tile issues the same number of requests.
 template <int ROWS_A, int ROWS_B, int WAVES>
-struct MxScaleFetch {
-    static constexpr int REQ_A = (ROWS_A + 63) / 64, REQ_B = (ROWS_B + 63) / 64;
-    static constexpr int PER = (REQ_A + REQ_B + WAVES - 1) / WAVES;
-    static constexpr int BYTES = PER * WAVES * 256;
-    static constexpr int B_OFFSET = REQ_A * 256;
-    unsigned off[PER];
-    bool is_b[PER];
-    __device__ __forceinline__ void init(const MxSide& a, const MxSide& b, int m0, int n0, int wave, int lane)
+struct MxScaleRing {
+    static constexpr int ROWS = ROWS_A + ROWS_B;
+    static constexpr int PER = (ROWS + 64 * WAVES - 1) / (64 * WAVES);   // requests of a wavefront per quarter
+    static constexpr int SLOT = 4 * PER * WAVES * 256, BYTES = 3 * SLOT;
+    static_assert(ROWS_A % 16 == 0, "a request serves lines of one operand");
+    const char *a_base, *b_base;    // scales of the tile's first lines from the slice's first block on
+    int a_lines, b_lines, row;
+    long pitch;                     // both operands have the same depth
+    unsigned off;
+    int dword;
+    __device__ __forceinline__ void init(const MxSide& a, const MxSide& b, int m0, int n0, int first, int lane)
     {
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-            const int req = wave + i * WAVES;
-            is_b[i] = req >= REQ_A;
-            const int row = (is_b[i] ? req - REQ_A : req) * 64 + lane;
-            const MxSide& s = is_b[i] ? b : a;
-            const int rows = is_b[i] ? ROWS_B : ROWS_A, first = is_b[i] ? n0 : m0;
-            off[i] = (row < rows && first + row < s.lines && s.blocks > 0) ? (unsigned)row * (unsigned)s.scale_pitch : NG_OOB_OFFSET;
-        }
+        a_base = a.scales + (long)m0 * a.scale_pitch + first;
+        b_base = b.scales + (long)n0 * b.scale_pitch + first;
+        a_lines = a.lines - m0;
+        b_lines = b.lines - n0;
+        pitch = a.scale_pitch;
+        row = lane >> 2;
+        dword = (lane & 3) * 4;
+        off = (unsigned)row * (unsigned)pitch + (unsigned)dword;
     }
-    // `first`: first block of the dword
-    __device__ __forceinline__ void issue(int i, const char* a_base, const char* b_base, int first, char* lds, int wave) const
+    // request i of quarter p of group `group`, `left` blocks of the lines from the group's
+    // first one on; dwords behind the last block are not read (they may lie behind the
+    // scales' memory)
+    __device__ __forceinline__ void issue(int p, int i, int group, int left, char* slot, int wave) const
     {
-        buffer_load_dword_to_lds(make_rsrc((is_b[i] ? b_base : a_base) + first), lds + (wave + i * WAVES) * 256, off[i]);
+        const int id = (p * PER + i) * WAVES + wave;
+        const bool is_b = id * 16 >= ROWS_A;
+        const int row0 = id * 16 - (is_b ? ROWS_A : 0);
+        const char* base = (is_b ? b_base : a_base) + row0 * pitch + group * 16;
+        int lines = (is_b ? b_lines : a_lines) - row0;
+        if (4 * PER * WAVES * 16 != ROWS) lines = id * 16 < ROWS ? lines : 0;
+        const bool there = (row < lines) & (dword < left);     // no branch: it would split the products' schedule
+        buffer_load_dword_to_lds(make_rsrc(base), slot + id * 256, there ? off : NG_OOB_OFFSET);
     }
 };
 
 // ---- fp4 . fp4 --------------------------------------------------------------------
-template <int BM, int BN, int WM, int WN, int NSTAGE, class Epi>
+template <int BM, int BN, int BK, int WM, int WN, int NSTAGE, class Epi>
 __global__ __launch_bounds__(WM * WN * 64)
 void mx44_kernel(MxSide a, MxSide b, Epi epi, CoreShape s)
 {
-    constexpr int BK = 128, LINE = BK / 2, NT = WM * WN * 64, WAVES = WM * WN;
+    constexpr int LINE = BK / 2, NT = WM * WN * 64, WAVES = WM * WN;
+    constexpr int STEPS = BK / 64, DW = BK / 128;            // matrix steps and scale dwords of a tile
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32, WTN = BN / WN;
     using TA = MxTile<BM, LINE>;
     using TB = MxTile<BN, LINE>;
-    using FA = MxFetch<TA, BM, NT, true>;
-    using FB = MxFetch<TB, BN, NT, true>;
-    using SF = MxScaleFetch<BM, BN, WAVES>;
-    constexpr int STAGE = TA::BYTES + TB::BYTES + SF::BYTES;
-    constexpr int SCALES = TA::BYTES + TB::BYTES;
-    constexpr int LOADS = FA::DATA + FB::DATA + SF::PER;     // requests of a wavefront per tile
+    using FA = MxFetch<TA, NT>;
+    using FB = MxFetch<TB, NT>;
+    using SF = MxScaleRing<BM, BN, WAVES>;
+    constexpr int STAGE = TA::BYTES + TB::BYTES;
+    constexpr int SCALES = NSTAGE * STAGE;
+    constexpr int SREQ = SF::PER * DW;                       // scale requests of a wavefront per tile
+    constexpr int LOADS = FA::DATA + FB::DATA + SREQ;        // all its requests
     constexpr int EPITCH = WTN * 4 + 16, EPI_BYTES = 32 * EPITCH;
-    constexpr int SMEM = NSTAGE * STAGE > EPI_BYTES * WAVES ? NSTAGE * STAGE : EPI_BYTES * WAVES;
+    constexpr int SMEM = SCALES + SF::BYTES > EPI_BYTES * WAVES ? SCALES + SF::BYTES : EPI_BYTES * WAVES;
     static_assert(SMEM <= 160 * 1024, "tile stages exceed the LDS of a compute unit");
     static_assert((NSTAGE - 1) * LOADS < 64, "the wait counter holds 6 bits");
     __shared__ __attribute__((aligned(16))) char smem[SMEM];
@@ -210,21 +224,18 @@ void mx44_kernel(MxSide a, MxSide b, Epi epi, CoreShape s)
     SF sf;
     fa.init(a, m0, t_begin, tid);
     fb.init(b, n0, t_begin, tid);
-    sf.init(a, b, m0, n0, wave, lane);
-    const char* a_scales = a.scales + (long)m0 * a.scale_pitch;
-    const char* b_scales = b.scales + (long)n0 * b.scale_pitch;
-    int g_block = t_begin * 4;
-    auto gissue = [&](int stage_off) {
-        char* st = smem + stage_off;
-#pragma unroll
-        for (int i = 0; i < SF::PER; i++) sf.issue(i, a_scales, b_scales, g_block, st + SCALES, wave);
-#pragma unroll
-        for (int i = 0; i < FA::DATA; i++) fa.issue(i, st, wave);
-#pragma unroll
-        for (int i = 0; i < FB::DATA; i++) fb.issue(i, st + TA::BYTES, wave);
+    sf.init(a, b, m0, n0, t_begin * (BK / 32), lane);
+    const int blocks = a.blocks - t_begin * (BK / 32);      // from this slice's first one on
+    // request q of a tile into the stage at st: its codes, and quarters p .. p + DW - 1 of a
+    // group of scales 8 dwords ahead
+    auto request = [&](int q, char* st, int p, int group, char* slot) {
+        if (q < FA::DATA) fa.issue(q, fa.lane_offset(), st, wave);
+        else if (q < FA::DATA + FB::DATA) fb.issue(q - FA::DATA, fb.lane_offset(), st + TA::BYTES, wave);
+        else if (q < LOADS) sf.issue(p + (q - FA::DATA - FB::DATA) / SF::PER, (q - FA::DATA - FB::DATA) % SF::PER, group, blocks - group * 16, slot, wave);
+    };
+    auto advance = [&]() {
         fa.advance();
         fb.advance();
-        g_block += 4;
     };
 
     float16_t acc[TM][TN];
@@ -235,91 +246,120 @@ void mx44_kernel(MxSide a, MxSide b, Epi epi, CoreShape s)
 #pragma unroll
             for (int v = 0; v < 16; v++) acc[i][j][v] = 0.0f;
 
-    // lane-constant addresses: block 2 st + half of the lane's line; the swizzle only
-    // depends on the line inside a block of 32
-    int a_off[TM], b_off[TN];
-#pragma unroll
-    for (int i = 0; i < TM; i++) a_off[i] = TA::offset((wm * TM + i) * 32 + row, half);
-#pragma unroll
-    for (int j = 0; j < TN; j++) b_off[j] = TA::BYTES + TB::offset((wn * TN + j) * 32 + row, half);
-    const int as_off = SCALES + (wm * TM * 32 + row) * 4, bs_off = SCALES + SF::B_OFFSET + (wn * TN * 32 + row) * 4;
+    // lane-constant addresses of block `half` of the lane's line; blocks of 32 lines lie a
+    // constant apart, and the step's chunk is an xor away (the swizzle distributes)
+    const int a_off = TA::offset(wm * TM * 32 + row, half), b_off = TA::BYTES + TB::offset(wn * TN * 32 + row, half);
+    const int as_off = SCALES + (wm * TM * 32 + row) * 16, bs_off = SCALES + (BM + wn * TN * 32 + row) * 16;
 
     uint4_t qa[2][TM], qb[2][TN];
-    int xa[2][TM], xb[2][TN];     // scales of a tile, this half's block of step 0 in byte 0, of step 1 in byte 2
-    auto load_step = [&](int stage_off, int st, uint4_t (&na)[TM], uint4_t (&nb)[TN]) {
-        const char* p = smem + stage_off;
+    // scales of this and the next tile: of a dword's four blocks this half's of the even
+    // step in byte 0, of the odd step in byte 2
+    int xa[DW][TM], xb[DW][TN];
+    unsigned ya[DW][TM], yb[DW][TN];
+    auto read_a = [&](const char* st, int step, int i) { return *reinterpret_cast<const uint4_t*>(st + (a_off ^ (step * 32)) + i * 32 * LINE); };
+    auto read_b = [&](const char* st, int step, int j) { return *reinterpret_cast<const uint4_t*>(st + (b_off ^ (step * 32)) + j * 32 * LINE); };
+    // scale dwords of the tile whose first dword is number d, from ring slot `slot` (a byte offset)
+    auto load_scales = [&](int slot, int d, unsigned (&na)[DW][TM], unsigned (&nb)[DW][TN]) {
 #pragma unroll
-        for (int i = 0; i < TM; i++) na[i] = *reinterpret_cast<const uint4_t*>(p + (a_off[i] ^ (st * 32)));
+        for (int w = 0; w < DW; w++) {
+            const char* p = smem + slot + ((d + w) & 3) * 4;
 #pragma unroll
-        for (int j = 0; j < TN; j++) nb[j] = *reinterpret_cast<const uint4_t*>(p + (b_off[j] ^ (st * 32)));
+            for (int i = 0; i < TM; i++) na[w][i] = *reinterpret_cast<const unsigned*>(p + as_off + i * 512);
+#pragma unroll
+            for (int j = 0; j < TN; j++) nb[w][j] = *reinterpret_cast<const unsigned*>(p + bs_off + j * 512);
+        }
     };
-    auto load_scales = [&](int stage_off, int first, int (&na)[TM], int (&nb)[TN]) {
-        const char* p = smem + stage_off;
-        const unsigned ma = mx_scale_mask(a.blocks, first);
+    auto take_scales = [&](int d) {
         const int shift = 8 * half;
 #pragma unroll
-        for (int i = 0; i < TM; i++) na[i] = (int)((*reinterpret_cast<const unsigned*>(p + as_off + i * 128) & ma) >> shift);
+        for (int w = 0; w < DW; w++) {
+            const unsigned mask = mx_scale_mask(blocks, (d + w) * 4);
 #pragma unroll
-        for (int j = 0; j < TN; j++) nb[j] = (int)((*reinterpret_cast<const unsigned*>(p + bs_off + j * 128) & ma) >> shift);
+            for (int i = 0; i < TM; i++) xa[w][i] = (int)((ya[w][i] & mask) >> shift);
+#pragma unroll
+            for (int j = 0; j < TN; j++) xb[w][j] = (int)((yb[w][j] & mask) >> shift);
+        }
     };
-    auto operand = [](const uint4_t& q) { return int8v_t{(int)q[0], (int)q[1], (int)q[2], (int)q[3], 0, 0, 0, 0}; };
-    auto multiply0 = [&](const uint4_t (&ca)[TM], const uint4_t (&cb)[TN], const int (&ea)[TM], const int (&eb)[TN]) {
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-            for (int j = 0; j < TN; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(ca[i]), operand(cb[j]), acc[i][j], 4, 4, 0, ea[i], 0, eb[j]);
-    };
-    auto multiply1 = [&](const uint4_t (&ca)[TM], const uint4_t (&cb)[TN], const int (&ea)[TM], const int (&eb)[TN]) {
-#pragma unroll
-        for (int i = 0; i < TM; i++)
-#pragma unroll
-            for (int j = 0; j < TN; j++)
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(operand(ca[i]), operand(cb[j]), acc[i][j], 4, 4, 2, ea[i], 2, eb[j]);
+    auto product = [&](int step, int i, int j) {
+        const int8v_t va{(int)qa[step & 1][i][0], (int)qa[step & 1][i][1], (int)qa[step & 1][i][2], (int)qa[step & 1][i][3], 0, 0, 0, 0};
+        const int8v_t vb{(int)qb[step & 1][j][0], (int)qb[step & 1][j][1], (int)qb[step & 1][j][2], (int)qb[step & 1][j][3], 0, 0, 0, 0};
+        const int ea = xa[step / 2][i], eb = xb[step / 2][j];
+        if ((step & 1) == 0) acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, acc[i][j], 4, 4, 0, ea, 0, eb);
+        else                 acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(va, vb, acc[i][j], 4, 4, 2, ea, 2, eb);
     };
 
+    // Requests run NSTAGE tiles ahead, past the last tile too: those fetch zeros (every
+    // chunk is out of range), so all tiles take the same path and the wait counts are
+    // constants.  Scales: all of group 0 and what of group 1 does not come with the first tiles.
+    static_assert(NSTAGE * DW <= 4, "the first tiles bring at most the four quarters of group 1");
+    auto next_slot = [&](int slot) { return slot == 2 * SF::SLOT ? 0 : slot + SF::SLOT; };
 #pragma unroll
-    for (int p = 0; p < NSTAGE; p++)
-        if (p < ntiles) gissue(p * STAGE);
-    if (ntiles >= NSTAGE) __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 1) * LOADS>::IMM);
-    else                  __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);
-    __syncthreads();
-    auto next_stage = [&](int off) { return (off + STAGE == NSTAGE * STAGE) ? 0 : off + STAGE; };
-    int rd = 0;
-    if (ntiles > 0) {
-        load_scales(0, t_begin * 4, xa[0], xb[0]);
-        load_step(0, 0, qa[0], qb[0]);
-    }
-    // one tile: step 0 with the reads of step 1 behind it, then the tile's barrier,
-    // then step 1 with the reads of the next tile behind it
-    auto tile = [&](int t, bool more, auto& cxa, auto& cxb, auto& nxa, auto& nxb, bool request, int vm_wait) {
-        load_step(rd, 1, qa[1], qb[1]);
-        multiply0(qa[0], qb[0], cxa, cxb);
-        if (!more) {
-            multiply1(qa[1], qb[1], cxa, cxb);
-            return;
+    for (int p = 0; p < 8 - NSTAGE * DW; p++)
+#pragma unroll
+        for (int i = 0; i < SF::PER; i++) {
+            const int q = p < 4 ? p : p - 4 + NSTAGE * DW, group = p < 4 ? 0 : 1;
+            sf.issue(q, i, group, blocks - group * 16, smem + SCALES + group * SF::SLOT, wave);
         }
-        if (vm_wait) __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
-        else         __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);
+#pragma unroll
+    for (int p = 0; p < NSTAGE; p++) {
+#pragma unroll
+        for (int q = 0; q < LOADS; q++) request(q, smem + p * STAGE, p * DW, 1, smem + SCALES + SF::SLOT);
+        advance();
+    }
+    __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 1) * LOADS>::IMM);
+    __syncthreads();
+    int rd = 0;
+    int read_slot = 0, write_slot = 2 * SF::SLOT;       // ring slots of the group read next and of the one requested now
+    load_scales(0, 0, ya, yb);
+    take_scales(0);
+#pragma unroll
+    for (int i = 0; i < TM; i++) qa[0][i] = read_a(smem, 0, i);
+#pragma unroll
+    for (int j = 0; j < TN; j++) qb[0][j] = read_b(smem, 0, j);
+
+    constexpr int N = TM * TN;
+    constexpr int REQ = (LOADS + N - 1) / N, READ = (TM + TN + N - 1) / N;
+    // A tile: all steps but the last with the fragment reads of the following step between
+    // the products; the barrier (behind it no wavefront reads this stage any more: the last
+    // step's fragments are in registers); the last step with the requests into the freed
+    // stage and the reads of the next tile between its products, so neither comes in a burst.
+    for (int t = 0; t < ntiles; t++) {
+#pragma unroll
+        for (int step = 0; step < STEPS - 1; step++)
+#pragma unroll
+            for (int p = 0; p < N; p++) {
+#pragma unroll
+                for (int q = p * READ; q < (p + 1) * READ; q++) {
+                    if (q < TM) qa[(step + 1) & 1][q < TM ? q : 0] = read_a(smem + rd, step + 1, q < TM ? q : 0);
+                    else if (q < TM + TN) qb[(step + 1) & 1][q >= TM && q < TM + TN ? q - TM : 0] = read_b(smem + rd, step + 1, q >= TM && q < TM + TN ? q - TM : 0);
+                }
+                product(step, p / TN, p % TN);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
-        const int freed = rd;
-        rd = next_stage(rd);
-        if (request) gissue(freed);
-        load_scales(rd, (t_begin + t + 1) * 4, nxa, nxb);
-        load_step(rd, 0, qa[0], qb[0]);
-        multiply1(qa[1], qb[1], cxa, cxb);
-    };
-    int t = 0;
-    for (; t + NSTAGE + 1 < ntiles; t += 2) {
-        tile(t, true, xa[0], xb[0], xa[1], xb[1], true, 1);
-        tile(t + 1, true, xa[1], xb[1], xa[0], xb[0], true, 1);
+        const int freed = rd, d = t * DW;
+        rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
+        if (((d + DW) & 3) == 0) read_slot = next_slot(read_slot);
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            product(STEPS - 1, p / TN, p % TN);
+            if (p == 0) load_scales(read_slot, d + DW, ya, yb);
+#pragma unroll
+            for (int q = p * READ; q < (p + 1) * READ; q++) {
+                if (q < TM) qa[0][q < TM ? q : 0] = read_a(smem + rd, 0, q < TM ? q : 0);
+                else if (q < TM + TN) qb[0][q >= TM && q < TM + TN ? q - TM : 0] = read_b(smem + rd, 0, q >= TM && q < TM + TN ? q - TM : 0);
+            }
+#pragma unroll
+            for (int q = p * REQ; q < (p + 1) * REQ; q++) request(q, smem + freed, d & 3, (d >> 2) + 2, smem + SCALES + write_slot);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        advance();
+        if (((d + DW) & 3) == 0) write_slot = next_slot(write_slot);
+        take_scales(d + DW);
     }
-    // the rest: at most NSTAGE + 1 tiles
-    for (; t < ntiles; t += 2) {
-        tile(t, t + 1 < ntiles, xa[0], xb[0], xa[1], xb[1], t + NSTAGE < ntiles, 0);
-        if (t + 1 < ntiles) tile(t + 1, t + 2 < ntiles, xa[1], xb[1], xa[0], xb[0], t + 1 + NSTAGE < ntiles, 0);
-    }
+    __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);    // nothing may land in LDS behind the next barrier
 
     __syncthreads();
     char* stage = smem + wave * EPI_BYTES;
@@ -327,144 +367,112 @@ void mx44_kernel(MxSide a, MxSide b, Epi epi, CoreShape s)
 }
 
 // ---- block scaled . fp16 -----------------------------------------------------------
-// One side's fragments.  A contraction tile is 64 values (two blocks); lanes 0..31
-// take the first block, lanes 32..63 the second, 8 values a step: the contraction
-// order inside a tile is a permutation both sides share.
-template <int FMT, int T> struct MxFrags;
-
-template <int T>
-struct MxFrags<NG_MX_NONE, T> {
-    static constexpr int LINE = 128;
-    half8_t v[2][T];
-    int off[T];
-    template <class Tile> __device__ __forceinline__ void init(int row0, int lane, int base)
+// A contraction tile is 64 values (two blocks): lanes 0..31 of a fragment take the
+// first block, lanes 32..63 the second, 8 values a step.  The contraction order inside
+// a tile is a permutation that both sides share.
+//
+// codes of one lane's block for the four steps of a tile, and their way to fp16 in two
+// halves of four values
+template <int FMT> struct MxBlock;
+template <> struct MxBlock<NG_MX_FP4> {
+    static constexpr int BYTES = 16;          // of a block
+    uint4_t raw;
+    float scale;
+    __device__ __forceinline__ void load(const char* p, int, unsigned byte)
     {
-#pragma unroll
-        for (int i = 0; i < T; i++) off[i] = base + Tile::offset(row0 + i * 32 + (lane & 31), (lane >> 5) * 4);
+        raw = *reinterpret_cast<const uint4_t*>(p);
+        scale = mx_scale_value(byte);
     }
-    __device__ __forceinline__ void load_tile(const char*, int, int, int, unsigned) {}
-    // chunk 4 half + step of the line: the xor with the swizzle distributes
-    __device__ __forceinline__ void load_step(const char* stage, int step, int to)
+    template <int STEP, int HALF> __device__ __forceinline__ void expand(half8_t& v) const
     {
-#pragma unroll
-        for (int i = 0; i < T; i++) v[to][i] = *reinterpret_cast<const half8_t*>(stage + (off[i] ^ (step * 16)));
+        const half2_t a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(raw[STEP], scale, 2 * HALF);
+        const half2_t b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(raw[STEP], scale, 2 * HALF + 1);
+        v[4 * HALF] = a[0]; v[4 * HALF + 1] = a[1]; v[4 * HALF + 2] = b[0]; v[4 * HALF + 3] = b[1];
     }
-    __device__ __forceinline__ half8_t get(int i, int step, int /*tile*/) const { return v[step & 1][i]; }
 };
-
-template <int T>
-struct MxFrags<NG_MX_FP4, T> {
-    static constexpr int LINE = 32;
-    uint4_t raw[2][T];
-    float scale[2][T];
-    int off[T], soff;
-    template <class Tile> __device__ __forceinline__ void init(int row0, int lane, int base)
+template <> struct MxBlock<NG_MX_INT8> {
+    static constexpr int BYTES = 32;
+    uint4_t raw[2];
+    MxInt8Scale scale;
+    // the second chunk of the block lies at p2 (the tile's swizzle has moved it)
+    __device__ __forceinline__ void load(const char* p, int to_second, unsigned byte)
     {
-#pragma unroll
-        for (int i = 0; i < T; i++) off[i] = base + Tile::offset(row0 + i * 32 + (lane & 31), lane >> 5);
+        raw[0] = *reinterpret_cast<const uint4_t*>(p);
+        raw[1] = *reinterpret_cast<const uint4_t*>(p + to_second);
+        scale = mx_int8_scale(byte);
     }
-    __device__ __forceinline__ void load_tile(const char* stage, int scales, int shift, int to, unsigned mask)
+    template <int STEP, int HALF> __device__ __forceinline__ void expand(half8_t& v) const
     {
-#pragma unroll
-        for (int i = 0; i < T; i++) {
-            raw[to][i] = *reinterpret_cast<const uint4_t*>(stage + off[i]);
-            scale[to][i] = mx_scale_value(((*reinterpret_cast<const unsigned*>(stage + scales + i * 128) & mask) >> shift) & 255u);
-        }
-    }
-    __device__ __forceinline__ void load_step(const char*, int, int) {}
-    __device__ __forceinline__ half8_t get(int i, int step, int tile) const { return mx_expand_fp4(raw[tile][i][step], scale[tile][i]); }
-};
-
-template <int T>
-struct MxFrags<NG_MX_INT8, T> {
-    static constexpr int LINE = 64;
-    uint4_t raw[2][T][2];
-    unsigned scale[2][T];
-    int off[T];
-    template <class Tile> __device__ __forceinline__ void init(int row0, int lane, int base)
-    {
-#pragma unroll
-        for (int i = 0; i < T; i++) off[i] = base + Tile::offset(row0 + i * 32 + (lane & 31), (lane >> 5) * 2);
-    }
-    __device__ __forceinline__ void load_tile(const char* stage, int scales, int shift, int to, unsigned mask)
-    {
-#pragma unroll
-        for (int i = 0; i < T; i++) {
-            raw[to][i][0] = *reinterpret_cast<const uint4_t*>(stage + off[i]);
-            raw[to][i][1] = *reinterpret_cast<const uint4_t*>(stage + (off[i] ^ 16));
-            scale[to][i] = ((*reinterpret_cast<const unsigned*>(stage + scales + i * 128) & mask) >> shift) & 255u;
-        }
-    }
-    __device__ __forceinline__ void load_step(const char*, int, int) {}
-    __device__ __forceinline__ half8_t get(int i, int step, int tile) const
-    {
-        const MxInt8Scale s = mx_int8_scale(scale[tile][i]);
-        const uint4_t& q = raw[tile][i][step >> 1];
-        half2_t a, b, c, d;
-        mx_expand_int8(q[(step & 1) * 2], s, a, b);
-        mx_expand_int8(q[(step & 1) * 2 + 1], s, c, d);
-        return half8_t{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+        half2_t a, b;
+        mx_expand_int8(raw[STEP / 2][(STEP & 1) * 2 + HALF], scale, a, b);
+        v[4 * HALF] = a[0]; v[4 * HALF + 1] = a[1]; v[4 * HALF + 2] = b[0]; v[4 * HALF + 3] = b[1];
     }
 };
 
-template <int FA_, int FB_, int BM, int BN, int WM, int WN, int NSTAGE, class Epi>
-__global__ __launch_bounds__(WM * WN * 64)
-void mxmix_kernel(MxSide a, MxSide b, Epi epi, CoreShape s)
+// X: the block-scaled operand (rows of C if X_IS_A, else its columns), D: the dense one.
+// WX x WD wavefronts; a wavefront expands BX / WX lines of codes and multiplies them
+// with BD / WD dense lines, so few X lines a wavefront mean little expansion.
+template <int FMT, bool X_IS_A, int BX, int BD, int WX, int WD, int NSTAGE, class Epi>
+__global__ __launch_bounds__(WX * WD * 64)
+void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
 {
-    constexpr int NT = WM * WN * 64, WAVES = WM * WN;
-    constexpr int TM = BM / WM / 32, TN = BN / WN / 32, WTN = BN / WN;
-    using GA = MxFrags<FA_, TM>;
-    using GB = MxFrags<FB_, TN>;
-    using TA = MxTile<BM, GA::LINE>;
-    using TB = MxTile<BN, GB::LINE>;
-    using FA = MxFetch<TA, BM, NT, FA_ != NG_MX_NONE>;
-    using FB = MxFetch<TB, BN, NT, FB_ != NG_MX_NONE>;
-    // only the block-scaled side has scales
-    constexpr int SROWS_A = FA_ != NG_MX_NONE ? BM : 0, SROWS_B = FB_ != NG_MX_NONE ? BN : 0;
-    using SF = MxScaleFetch<SROWS_A, SROWS_B, WAVES>;
-    constexpr int SCALES = TA::BYTES + TB::BYTES;
-    constexpr int STAGE = SCALES + SF::BYTES;
-    constexpr int LOADS = FA::DATA + FB::DATA + SF::PER;
+    constexpr int NT = WX * WD * 64, WAVES = WX * WD;
+    constexpr int TX = BX / WX / 32, TD = BD / WD / 32;
+    constexpr int BM = X_IS_A ? BX : BD, BN = X_IS_A ? BD : BX;
+    constexpr int TM = X_IS_A ? TX : TD, TN = X_IS_A ? TD : TX, WTN = TN * 32;
+    using Block = MxBlock<FMT>;
+    using TileX = MxTile<BX, 2 * Block::BYTES>;
+    using TileD = MxTile<BD, 128>;
+    using FX = MxFetch<TileX, NT>;
+    using FD = MxFetch<TileD, NT>;
+    // scales: groups of 16 blocks (8 tiles), four lanes a line, in a ring of two slots
+    constexpr int SPER = BX / 16 / WAVES, SLOT = BX * 16;
+    static_assert(BX % (16 * WAVES) == 0 && SPER <= 4, "scale requests must divide evenly over wavefronts");
+    constexpr int STAGE = TileX::BYTES + TileD::BYTES, SCALES = NSTAGE * STAGE;
+    constexpr int LOADS = FX::DATA + FD::DATA;
     constexpr int EPITCH = WTN * 4 + 16, EPI_BYTES = 32 * EPITCH;
-    constexpr int SMEM = NSTAGE * STAGE > EPI_BYTES * WAVES ? NSTAGE * STAGE : EPI_BYTES * WAVES;
+    constexpr int SMEM = SCALES + 2 * SLOT > EPI_BYTES * WAVES ? SCALES + 2 * SLOT : EPI_BYTES * WAVES;
     static_assert(SMEM <= 160 * 1024, "tile stages exceed the LDS of a compute unit");
     static_assert((NSTAGE - 1) * LOADS < 64, "the wait counter holds 6 bits");
-    static_assert((FA_ == NG_MX_NONE) != (FB_ == NG_MX_NONE), "one side is block scaled");
     __shared__ __attribute__((aligned(16))) char smem[SMEM];
 
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int wm = wave % WM, wn = wave / WM;
+    const int wx = wave % WX, wd = wave / WX;
+    const int half = lane >> 5, row = lane & 31;
 
     int tm, tn, split;
     if (!block_work(s, tm, tn, split)) return;
     const int m0 = tm * BM, n0 = tn * BN;
+    const int x0 = X_IS_A ? m0 : n0, d0 = X_IS_A ? n0 : m0;
     const int per = (s.k_tiles + s.splits - 1) / s.splits;
     const int t_begin = split * per, t_end = min(t_begin + per, s.k_tiles);
     const int ntiles = t_end - t_begin;
 
-    FA fa;
-    FB fb;
-    SF sf;
-    fa.init(a, m0, t_begin, tid);
-    fb.init(b, n0, t_begin, tid);
-    sf.init(a, b, m0, n0, wave, lane);
-    const char* a_scales = FA_ != NG_MX_NONE ? a.scales + (long)m0 * a.scale_pitch : nullptr;
-    const char* b_scales = FB_ != NG_MX_NONE ? b.scales + (long)n0 * b.scale_pitch : nullptr;
-    const int blocks = FA_ != NG_MX_NONE ? a.blocks : b.blocks;
-    int g_tile = t_begin;
-    auto gissue = [&](int stage_off) {
-        char* st = smem + stage_off;
-        // two tiles share a dword of scales
-#pragma unroll
-        for (int i = 0; i < SF::PER; i++) sf.issue(i, a_scales, b_scales, (2 * g_tile) & ~3, st + SCALES, wave);
-#pragma unroll
-        for (int i = 0; i < FA::DATA; i++) fa.issue(i, st, wave);
-#pragma unroll
-        for (int i = 0; i < FB::DATA; i++) fb.issue(i, st + TA::BYTES, wave);
-        fa.advance();
-        fb.advance();
-        g_tile++;
+    FX fx;
+    FD fd;
+    fx.init(x, x0, t_begin, tid);
+    fd.init(d, d0, t_begin, tid);
+    auto request = [&](int q, char* st) {
+        if (q < FX::DATA) fx.issue(q, fx.lane_offset(), st, wave);
+        else if (q < LOADS) fd.issue(q - FX::DATA, fd.lane_offset(), st + TileX::BYTES, wave);
+    };
+    auto advance = [&]() {
+        fx.advance();
+        fd.advance();
+    };
+    const int first = (2 * t_begin) & ~3;             // a dword of scales holds two tiles
+    const int s_skip = 2 * t_begin - first;           // 0, or 2 where the slice starts inside a dword
+    const int blocks = x.blocks - first;
+    const char* s_base = x.scales + (long)x0 * x.scale_pitch + first;
+    const unsigned s_off = (unsigned)(lane >> 2) * (unsigned)x.scale_pitch + (unsigned)(lane & 3) * 4u;
+    // 16 lines of group `group`; dwords behind the last block are not read (they may lie
+    // behind the scales' memory)
+    auto request_scales = [&](int i, int group) {
+        const int line = (i * WAVES + wave) * 16;
+        const bool there = ((lane >> 2) < x.lines - x0 - line) & ((lane & 3) * 4 < blocks - group * 16);
+        buffer_load_dword_to_lds(make_rsrc(s_base + line * x.scale_pitch + group * 16), smem + SCALES + (group & 1) * SLOT + line * 16,
+                                 there ? s_off : NG_OOB_OFFSET);
     };
 
     float16_t acc[TM][TN];
@@ -475,82 +483,114 @@ void mxmix_kernel(MxSide a, MxSide b, Epi epi, CoreShape s)
 #pragma unroll
             for (int v = 0; v < 16; v++) acc[i][j][v] = 0.0f;
 
-    GA ga;
-    GB gb;
-    ga.template init<TA>(wm * TM * 32, lane, 0);
-    gb.template init<TB>(wn * TN * 32, lane, TA::BYTES);
-    const int as_off = SCALES + (wm * TM * 32 + (lane & 31)) * 4;
-    const int bs_off = SCALES + SF::B_OFFSET + (wn * TN * 32 + (lane & 31)) * 4;
-    auto load_tile = [&](int stage_off, int kt, int to) {
-        const char* p = smem + stage_off;
-        const unsigned mask = mx_scale_mask(blocks, (2 * kt) & ~3);
-        const int shift = 8 * (((2 * kt) & 2) + (lane >> 5));
-        ga.load_tile(p, as_off, shift, to, mask);
-        gb.load_tile(p, bs_off, shift, to, mask);
-    };
-    auto load_step = [&](int stage_off, int step) {
-        const char* p = smem + stage_off;
-        ga.load_step(p, step, step & 1);
-        gb.load_step(p, step, step & 1);
-    };
-    auto multiply = [&](int step, int tile) {
-        half8_t fb_[TN];
-#pragma unroll
-        for (int j = 0; j < TN; j++) fb_[j] = gb.get(j, step, tile);
-#pragma unroll
-        for (int i = 0; i < TM; i++) {
-            const half8_t fa_ = ga.get(i, step, tile);
-#pragma unroll
-            for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa_, fb_[j], acc[i][j], 0, 0, 0);
-        }
-    };
+    constexpr int XC = Block::BYTES / 16;             // chunks of a block
+    const int x_off = TileX::offset(wx * TX * 32 + row, half * XC);
+    const int x_second = XC == 2 ? TileX::offset(row, half * XC + 1) - TileX::offset(row, half * XC) : 0;
+    const int d_off = TileX::BYTES + TileD::offset(wd * TD * 32 + row, half * 4);
+    const int s_read = SCALES + (wx * TX * 32 + row) * 16 + half;
 
+    Block blk[TX];
+    half8_t fx_[2][TX], fd_[2][TD];
+    // codes and scales of tile t (counted from the slice's first)
+    auto load_blocks = [&](int stage_off, int t, int i) {
+        const int b = s_skip + 2 * t;                  // of the tile's first block
+        const unsigned byte = *reinterpret_cast<const unsigned char*>(smem + s_read + ((b >> 4) & 1) * SLOT + i * 512 + (b & 15));
+        blk[i].load(smem + stage_off + x_off + i * 64 * Block::BYTES, x_second, b + half < blocks ? byte : 0u);
+    };
+    // dense chunk 4 half + step of the line: the xor with the swizzle distributes
+    auto load_dense = [&](int stage_off, int step, int to, int i) {
+        fd_[to][i] = *reinterpret_cast<const half8_t*>(smem + stage_off + (d_off ^ (step * 16)) + i * 32 * 128);
+    };
+    auto product = [&](int step, int p) {
+        const int i = p / TN, j = p % TN;
+        if constexpr (X_IS_A) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fx_[step & 1][i], fd_[step & 1][j], acc[i][j], 0, 0, 0);
+        else                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fd_[step & 1][i], fx_[step & 1][j], acc[i][j], 0, 0, 0);
+    };
+    // piece c (half of a line's 8 values) of a step's expansion
+    auto expand0 = [&](int c) { if (c & 1) blk[c / 2].template expand<0, 1>(fx_[0][c / 2]); else blk[c / 2].template expand<0, 0>(fx_[0][c / 2]); };
+    auto expand1 = [&](int c) { if (c & 1) blk[c / 2].template expand<1, 1>(fx_[1][c / 2]); else blk[c / 2].template expand<1, 0>(fx_[1][c / 2]); };
+    auto expand2 = [&](int c) { if (c & 1) blk[c / 2].template expand<2, 1>(fx_[0][c / 2]); else blk[c / 2].template expand<2, 0>(fx_[0][c / 2]); };
+    auto expand3 = [&](int c) { if (c & 1) blk[c / 2].template expand<3, 1>(fx_[1][c / 2]); else blk[c / 2].template expand<3, 0>(fx_[1][c / 2]); };
+
+    // Requests run NSTAGE tiles ahead, past the last tile too: those fetch zeros (every
+    // chunk is out of range), so all tiles take the same path.  The waits count the codes'
+    // and the dense requests only; where scale requests lie between them, they wait for a little more.
 #pragma unroll
-    for (int p = 0; p < NSTAGE; p++)
-        if (p < ntiles) gissue(p * STAGE);
-    if (ntiles >= NSTAGE) __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 1) * LOADS>::IMM);
-    else                  __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);
-    __syncthreads();
-    auto next_stage = [&](int off) { return (off + STAGE == NSTAGE * STAGE) ? 0 : off + STAGE; };
-    int rd = 0;
-    if (ntiles > 0) {
-        load_tile(0, t_begin, 0);
-        load_step(0, 0);
+    for (int i = 0; i < SPER; i++) request_scales(i, 0);
+#pragma unroll
+    for (int p = 0; p < NSTAGE; p++) {
+#pragma unroll
+        for (int q = 0; q < LOADS; q++) request(q, smem + p * STAGE);
+        advance();
     }
-    auto tile = [&](int t, bool more, int cur, bool request, int vm_wait) {
+    __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 1) * LOADS>::IMM);
+    __syncthreads();
+    int rd = 0;
 #pragma unroll
-        for (int st = 0; st < 3; st++) {
-            load_step(rd, st + 1);
-            multiply(st, cur);
-        }
-        if (!more) {
-            multiply(3, cur);
-            return;
-        }
-        if (vm_wait) __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
-        else         __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);
+    for (int i = 0; i < TX; i++) load_blocks(0, 0, i);
+#pragma unroll
+    for (int i = 0; i < TD; i++) load_dense(0, 0, 0, i);
+#pragma unroll
+    for (int c = 0; c < 2 * TX; c++) expand0(c);
+
+    constexpr int N = TM * TN;
+    constexpr int REQ = (LOADS + N - 1) / N, READ = (TD + N - 1) / N, PIECES = (2 * TX + N - 1) / N;
+    constexpr int TAIL = N / 2, TAIL_PIECES = (2 * TX + (N - TAIL) - 1) / (N - TAIL);
+    for (int t = 0; t < ntiles; t++) {
+        // steps 0 .. 2, each with the dense reads and the expansion of the next between its products
+#pragma unroll
+        for (int step = 0; step < 3; step++)
+#pragma unroll
+            for (int p = 0; p < N; p++) {
+#pragma unroll
+                for (int q = p * READ; q < (p + 1) * READ; q++)
+                    if (q < TD) load_dense(rd, step + 1, (step + 1) & 1, q < TD ? q : 0);
+                product(step, p);
+#pragma unroll
+                for (int c = p * PIECES; c < (p + 1) * PIECES; c++)
+                    if (c < 2 * TX) {
+                        if (step == 0) expand1(c < 2 * TX ? c : 0);
+                        else if (step == 1) expand2(c < 2 * TX ? c : 0);
+                        else expand3(c < 2 * TX ? c : 0);
+                    }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
         __syncthreads();
         __builtin_amdgcn_sched_barrier(0);
-        const int freed = rd;
-        rd = next_stage(rd);
-        if (request) gissue(freed);
-        load_tile(rd, t_begin + t + 1, cur ^ 1);
-        load_step(rd, 0);
-        multiply(3, cur);
-    };
-    int t = 0;
-    for (; t + NSTAGE + 1 < ntiles; t += 2) {
-        tile(t, true, 0, true, 1);
-        tile(t + 1, true, 1, true, 1);
+        const int freed = rd, b = s_skip + 2 * t;
+        rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
+        // the group after this one, one request at each of its first tiles (the slot's last
+        // group has been read: the tile before this group took its scales two barriers ago)
+        if ((b & 15) / 2 - (s_skip && b < 16 ? 1 : 0) < SPER) request_scales((b & 15) / 2 - (s_skip && b < 16 ? 1 : 0), (b >> 4) + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        // last step: the next tile's codes first, the requests into the freed stage, the
+        // next tile's dense reads, and in the second half its first expansion
+#pragma unroll
+        for (int i = 0; i < TX; i++) load_blocks(rd, t + 1, i);
+#pragma unroll
+        for (int p = 0; p < N; p++) {
+            product(3, p);
+#pragma unroll
+            for (int q = p * READ; q < (p + 1) * READ; q++)
+                if (q < TD) load_dense(rd, 0, 0, q < TD ? q : 0);
+#pragma unroll
+            for (int q = p * REQ; q < (p + 1) * REQ; q++) request(q, smem + freed);
+            if (p >= TAIL) {
+#pragma unroll
+                for (int c = (p - TAIL) * TAIL_PIECES; c < (p - TAIL + 1) * TAIL_PIECES; c++)
+                    if (c < 2 * TX) expand0(c < 2 * TX ? c : 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        advance();
     }
-    for (; t < ntiles; t += 2) {
-        tile(t, t + 1 < ntiles, 0, t + NSTAGE < ntiles, 0);
-        if (t + 1 < ntiles) tile(t + 1, t + 2 < ntiles, 1, t + 1 + NSTAGE < ntiles, 0);
-    }
+    __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);    // nothing may land in LDS behind the next barrier
 
     __syncthreads();
     char* stage = smem + wave * EPI_BYTES;
-    EpilogueBands<TM, TN, WTN, EPITCH, 0>::run(acc, stage, lane, m0 + wm * (BM / WM), n0 + wn * WTN, 0, split, epi);
+    const int wm = X_IS_A ? wx : wd, wn = X_IS_A ? wd : wx;
+    EpilogueBands<TM, TN, WTN, EPITCH, 0>::run(acc, stage, lane, m0 + wm * TM * 32, n0 + wn * WTN, 0, split, epi);
 }
 
 }  // namespace ng

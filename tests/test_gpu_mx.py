@@ -182,6 +182,24 @@ def test_fp4_product(ng, m, n, k, out):
     _check_product(C.get(), a, b, "fp4 %s" % ((m, n, k),), relu=m % 2 == 0)
 
 
+@pytest.mark.parametrize("kinds", ["44", "4h", "h4", "8h", "h8"])
+@pytest.mark.parametrize("m,n,k", [(530, 1030, 1100), (2900, 3080, 300)])
+def test_larger_products(ng, kinds, m, n, k):
+    """several tiles in both directions, ragged; the second fills the chip"""
+    rng = np.random.default_rng(k)
+    def side(kind, shape, axis):
+        if kind == "h":
+            x = rng.standard_normal(shape).astype(np.float16)
+            return ng.array(x), x
+        return _operand(ng, rng, shape, "fp4" if kind == "4" else "int8", axis)
+    A, a = side(kinds[0], (m, k), 1)
+    B, b = side(kinds[1], (k, n), 0)
+    for out in (np.float16, np.float32):
+        C = ng.empty((m, n), dtype=out)
+        ng.mx_dot(A, B, C)
+        _check_product(C.get(), a.astype(np.float64), b.astype(np.float64), kinds)
+
+
 MIX = [("fp4", "left"), ("fp4", "right"), ("int8", "left"), ("int8", "right")]
 
 
