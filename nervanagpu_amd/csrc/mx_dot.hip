@@ -1,5 +1,5 @@
 // Products of block-scaled matrices: C = round(beta*C + relu(alpha * A.B)).
-#include "mx_gemm.h"
+#include "mx_skinny.h"
 
 #include <algorithm>
 
@@ -24,6 +24,24 @@ void mx_pack_kernel(const unsigned short* __restrict__ X, long ld, int along, in
 #pragma unroll 4
     for (int j = ty; j < 64; j += 4)
         if (line0 + j < lines && i0 + tx < padded) out[(long)(line0 + j) * padded + i0 + tx] = tile[j][tx];
+}
+
+// The same for few lines: a thread takes 8 values of one line, neighbouring threads
+// neighbouring lines (rows of X with along = 0)
+__global__ __launch_bounds__(256)
+void mx_pack_few_kernel(const unsigned short* __restrict__ X, long ld, int along, int lines, int depth, int padded,
+                        unsigned short* __restrict__ out)
+{
+    const long id = (long)blockIdx.x * 256 + threadIdx.x;
+    const int groups = padded / 8;
+    const int line = (int)(id % lines), g = (int)(id / lines);
+    if (g >= groups) return;
+    unsigned short v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = g * 8 + i < depth ? X[along ? (long)line * ld + g * 8 + i : (long)(g * 8 + i) * ld + line] : (unsigned short)0;
+    uint4_t w;
+    __builtin_memcpy(&w, v, 16);
+    *reinterpret_cast<uint4_t*>(out + (long)line * padded + g * 8) = w;
 }
 
 struct MxArgs {
@@ -52,7 +70,8 @@ static size_t pack_bytes(const ng_mx_operand& o, int lines, int k)
     return align_up((size_t)lines * padded_depth(k) * 2, 256);
 }
 
-struct MxPlan { int bm, bn, bk, splits; };
+// skinny: groups of 16 dense lines of the kernel for few of them, 0 for tiles
+struct MxPlan { int bm, bn, bk, splits, skinny; };
 
 // as many slices of the contraction as give about one workgroup per CU, each at least
 // `least` tiles deep
@@ -72,14 +91,23 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
 {
     const int cus = device_cu_count();
     auto tiles = [&](int bm, int bn) { return (long)ceil_div(m, bm) * ceil_div(n, bn); };
-    MxPlan p{128, 128, 64, 1};
+    MxPlan p{128, 128, 64, 1, 0};
     int least = 4;
+    if (!is_44(A, B) && (A.format == NG_MX_FP4 || B.format == NG_MX_FP4)) {
+        const int dense_lines = A.format == NG_MX_NONE ? m : n;
+        if (dense_lines <= 32) {
+            p.skinny = (dense_lines + 15) / 16;
+            return p;
+        }
+    }
     if (is_44(A, B)) {
         p.bk = 256;
         least = 2;
         if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2) p.bm = p.bn = 256;
         else if (tiles(128, 128) <= cus / 2) p.bm = p.bn = 64;
-    } else if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2) {
+    } else if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2 && k > 256) {
+        // a contraction of few tiles is all prologue and store: more, smaller workgroups overlap
+        // those (9216x4096 outputs of k = 128: 48 us on 256x256 tiles, 35 us on 128x128 with two stages)
         p.bm = p.bn = 256;
     }
     const int out_tiles = (int)std::min<long>(tiles(p.bm, p.bn), 1 << 30);
@@ -128,8 +156,25 @@ static void launch_tiles(const MxArgs& g, const MxPlan& p, const MxSide& a, cons
         constexpr int FMT = X_IS_A ? FA : FB;
         const MxSide &x = X_IS_A ? a : b, &d = X_IS_A ? b : a;
         if (p.bm == 256) hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 256, 256, 4, 2, 3, Epi>), grid, dim3(512), 0, g.stream, x, d, epi, s);
+        else if (s.k_tiles <= 2) hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 128, 128, 2, 2, 2, Epi>), grid, dim3(256), 0, g.stream, x, d, epi, s);
         else             hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, x, d, epi, s);
     }
+}
+
+template <bool X_IS_A, class Epi>
+static int launch_skinny(const MxArgs& g, int groups, const MxSide& x, const MxSide& d, const Epi& epi)
+{
+    const dim3 grid((unsigned)ceil_div(x.lines, 16));
+    // sixteen wavefronts keep more of a long line in flight
+    const bool deep = x.blocks >= 256;
+#define NG_SKINNY(NC, WAVES)                                                                                              \
+    hipLaunchKernelGGL((mx_skinny_kernel<X_IS_A, NC, WAVES, Epi>), grid, dim3(WAVES * 64), 0, g.stream, x, d, epi, x.lines, \
+                       d.lines, d.chunks)
+    if (groups == 1) { if (deep) NG_SKINNY(1, 16); else NG_SKINNY(1, 4); }
+    else             { if (deep) NG_SKINNY(2, 8); else NG_SKINNY(2, 4); }
+#undef NG_SKINNY
+    NG_CHECK_LAUNCH("mx product of few lines");
+    return 0;
 }
 
 template <typename T, int FA, int FB>
@@ -149,6 +194,9 @@ static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
     ScaleStoreEpilogue<T> epi{(T*)g.C, 0, g.ldc, g.m, g.n, g.alpha, g.beta, (g.flags & NG_FLAG_RELU) ? 1u : 0u,
                               mx_sr_bits(g.flags, g.c_dtype), g.seed, g.rng_stream,
                               (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u};
+    if constexpr ((FA == NG_MX_FP4) != (FB == NG_MX_FP4)) {
+        if (p.skinny) return launch_skinny<FA == NG_MX_FP4>(g, p.skinny, FA == NG_MX_FP4 ? a : b, FA == NG_MX_FP4 ? b : a, epi);
+    }
     if (s.splits == 1) {
         launch_tiles<T, FA, FB>(g, p, a, b, epi, s, grid);
         NG_CHECK_LAUNCH("mx product");
@@ -239,9 +287,13 @@ int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const n
         if (bytes && k) {
             end -= bytes;
             const int padded = padded_depth(k);
-            if (ceil_div(k, 64) > 65535) return fail(-98, "ng_mx_gemm: contraction too long");
-            hipLaunchKernelGGL(mx_pack_kernel, dim3((unsigned)ceil_div(lines, 64), (unsigned)ceil_div(padded, 64)), dim3(256), 0,
-                               g.stream, (const unsigned short*)o->codes, o->ld, o->along, lines, k, padded, (unsigned short*)end);
+            const unsigned short* from = (const unsigned short*)o->codes;
+            if (lines <= 64)
+                hipLaunchKernelGGL(mx_pack_few_kernel, dim3((unsigned)(((long)lines * (padded / 8) + 255) / 256)), dim3(256), 0, g.stream,
+                                   from, o->ld, o->along, lines, k, padded, (unsigned short*)end);
+            else
+                hipLaunchKernelGGL(mx_pack_kernel, dim3((unsigned)ceil_div(lines, 64), (unsigned)ceil_div(padded, 64)), dim3(256), 0,
+                                   g.stream, from, o->ld, o->along, lines, k, padded, (unsigned short*)end);
             NG_CHECK_LAUNCH("mx pack");
             o->codes = end;
             o->along = 1;

@@ -26,6 +26,7 @@ inline long mx_code_pitch(int fmt, int depth) { return (long)mx_blocks(depth) * 
 inline long mx_scale_pitch(int depth) { return (long)((mx_blocks(depth) + 7) / 8) * 8; }
 
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
 
 // maximum over the four lanes of a quad (two lane permutes on the vector unit)
 NG_DEV unsigned mx_quad_max(unsigned v)
@@ -63,16 +64,18 @@ NG_DEV float mx_scale_value(unsigned byte)
 // high and the low half of word i (as the fp16 stores' stochastic rounding does)
 NG_DEV unsigned mx_random16(unsigned word, bool odd) { return odd ? (word & 0xFFFFu) : (word >> 16); }
 
-// |x| * 2^-e (below 8 for fp4) -> code by adding a uniform fraction of the local
-// unit and truncating.  Fixed point with 15 bits: the unit is 2^14 below 2, 2^15
-// below 4 and 2^16 above; values of one unit are consecutive codes, so the code is
-// the truncated quotient plus the first code of the range.
+// |x| * 2^-e (at most 6) -> code by adding a uniform fraction of the local unit and
+// truncating: T = floor(|x| 2^-e 2^15); the unit is 2^14 below 2, 2^15 below 4 and 2^16
+// above, the random number the top 14, 15 or 16 of the 16 bits.  In the fp32 pattern of T
+// all three units are the same place, bit 22, so one addition serves them: what the
+// pattern of T leaves free below its last bit takes the random bits that do not count.
+// Below 1, where the unit stays 2^14, T + 2^15 takes its place: [1, 2) two codes up.
 NG_DEV unsigned mx_fp4_stochastic(float a, unsigned r16)
 {
     const unsigned T = (unsigned)(a * 32768.0f);
-    const unsigned bits = T < 65536u ? 14u : T < 131072u ? 15u : 16u;
-    const unsigned code = ((T + (r16 >> (16u - bits))) >> bits) + 2u * (bits - 14u);
-    return min(code, 7u);
+    const bool low = T < 32768u;
+    const unsigned bits = __float_as_uint((float)(low ? T + 32768u : T));
+    return ((bits + (r16 << 6)) >> 22) - (low ? 284u : 282u);
 }
 
 NG_DEV unsigned mx_int8_magnitude_stochastic(float a, unsigned r16)
@@ -136,13 +139,13 @@ NG_DEV void mx_decode8(const unsigned (&in)[2], unsigned scale_byte, float (&v)[
 {
     const float s = mx_scale_value(scale_byte);
     if constexpr (FMT == NG_MX_FP4) {
+        const float2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[0], 1.0f, 0);
+        const float2_t b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[0], 1.0f, 1);
+        const float2_t c = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[0], 1.0f, 2);
+        const float2_t d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(in[0], 1.0f, 3);
+        const float grid[8] = {a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            const unsigned q = (in[0] >> (4 * i)) & 7u;
-            // codes 0..3 are halves; 4 and 5 units above 2; 6 and 7 steps of 2 above 4
-            const float m = q < 4u ? 0.5f * (float)q : q < 6u ? (float)(q - 2u) : (float)(2u * q - 8u);
-            v[i] = __uint_as_float(__float_as_uint(m) | ((in[0] << (28 - 4 * i)) & 0x80000000u)) * s;
-        }
+        for (int i = 0; i < 8; i++) v[i] = grid[i] * s;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; i++) {

@@ -315,6 +315,30 @@ inline emu_float16_t __builtin_amdgcn_mfma_f32_32x32x2f32(float a, float b, emu_
     return c;
 }
 
+typedef float emu_float4_t __attribute__((ext_vector_type(4)));
+// D = A (16 x 32) . B (32 x 16) + C: lane l holds row / column l & 15 and contraction values
+// 8 (l >> 4) .. + 7 of A / B, and column l & 15, rows 4 (l >> 4) + v of C / D
+inline emu_float4_t __builtin_amdgcn_mfma_f32_16x16x32_f16(emu_half8_t a, emu_half8_t b, emu_float4_t c, int, int, int)
+{
+    char* slots = emu::wave_exchange_begin();
+    std::memcpy(slots + 64 * emu::cur->lane, &a, 16);
+    std::memcpy(slots + 64 * emu::cur->lane + 16, &b, 16);
+    emu::wave_exchange_sync();
+    const int lane = emu::cur->lane, col = lane & 15;
+    for (int v = 0; v < 4; v++) {
+        const int row = 4 * (lane >> 4) + v;
+        float sum = 0.0f;
+        for (int k = 0; k < 32; k++) {
+            _Float16 av, bv;
+            std::memcpy(&av, slots + 64 * (row + 16 * (k / 8)) + 2 * (k % 8), 2);
+            std::memcpy(&bv, slots + 64 * (col + 16 * (k / 8)) + 16 + 2 * (k % 8), 2);
+            sum += (float)av * (float)bv;
+        }
+        c[v] += sum;
+    }
+    return c;
+}
+
 // ---- lane permutes, byte permutes ----------------------------------------------------------
 // quad permutes only (control below 256): lane 4q + i reads lane 4q + (control >> 2i & 3)
 inline int __builtin_amdgcn_update_dpp(int, int v, int control, int, int, bool)
@@ -363,6 +387,14 @@ inline emu_half2_t __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(unsigned w, float sc
     emu_half2_t r = {(_Float16)(emu_fp4_value(v & 15) * scale), (_Float16)(emu_fp4_value(v >> 4) * scale)};
     return r;
 }
+typedef float emu_float2_t __attribute__((ext_vector_type(2)));
+inline emu_float2_t __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(unsigned w, float scale, int byte)
+{
+    const unsigned v = (w >> (8 * byte)) & 255u;
+    emu_float2_t r = {emu_fp4_value(v & 15) * scale, emu_fp4_value(v >> 4) * scale};
+    return r;
+}
+inline float __builtin_amdgcn_exp2f(float x) { return std::exp2(x); }
 inline float emu_e8m0(int byte) { return byte == 255 ? NAN : std::ldexp(1.0f, byte - 127); }
 typedef int emu_int8v_t __attribute__((ext_vector_type(8)));
 // D = A (32 x 64) . B (64 x 32) + C of 4-bit operands (formats 4): lane l holds contraction values
