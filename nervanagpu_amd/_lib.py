@@ -18,6 +18,7 @@ COMMON_HEADER = os.path.join(_HERE, "csrc", "ng_device_common.h")
 
 NG_F16, NG_F32, NG_U8, NG_I8 = 0, 1, 2, 3
 NG_MX_NONE, NG_MX_FP4, NG_MX_INT8 = 0, 1, 2
+NG_MX_WORKSPACE = -102      # ng_mx_gemm: the workspace is too small, nothing was launched
 FLAG_SR, FLAG_RELU = 1, 2
 
 

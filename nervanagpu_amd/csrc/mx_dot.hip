@@ -26,24 +26,6 @@ void mx_pack_kernel(const unsigned short* __restrict__ X, long ld, int along, in
         if (line0 + j < lines && i0 + tx < padded) out[(long)(line0 + j) * padded + i0 + tx] = tile[j][tx];
 }
 
-// The same for few lines: a thread takes 8 values of one line, neighbouring threads
-// neighbouring lines (rows of X with along = 0)
-__global__ __launch_bounds__(256)
-void mx_pack_few_kernel(const unsigned short* __restrict__ X, long ld, int along, int lines, int depth, int padded,
-                        unsigned short* __restrict__ out)
-{
-    const long id = (long)blockIdx.x * 256 + threadIdx.x;
-    const int groups = padded / 8;
-    const int line = (int)(id % lines), g = (int)(id / lines);
-    if (g >= groups) return;
-    unsigned short v[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = g * 8 + i < depth ? X[along ? (long)line * ld + g * 8 + i : (long)(g * 8 + i) * ld + line] : (unsigned short)0;
-    uint4_t w;
-    __builtin_memcpy(&w, v, 16);
-    *reinterpret_cast<uint4_t*>(out + (long)line * padded + g * 8) = w;
-}
-
 struct MxArgs {
     int c_dtype, m, n, k;
     ng_mx_operand A, B;
@@ -58,15 +40,27 @@ static int ceil_div(int a, int b) { return (a + b - 1) / b; }
 
 static int padded_depth(int k) { return ceil_div(k, 8) * 8; }
 
-// a dense operand that the kernels can read where it lies
-static bool dense_in_place(const ng_mx_operand& o, int lines, int k)
+// a dense operand that the kernels can read where it lies: whole 16-byte chunks, along
+// the contraction, or (right operand of a fp4 one) across it
+static bool dense_in_place(const ng_mx_operand& o, const ng_mx_operand* left, int lines, int k)
 {
-    return o.along && ((uintptr_t)o.codes & 15) == 0 && k % 8 == 0 && (lines <= 1 || (o.ld % 8 == 0 && o.ld < (1L << 21)));
+    if (((uintptr_t)o.codes & 15) != 0) return false;
+    if (o.along) return k % 8 == 0 && (lines <= 1 || (o.ld % 8 == 0 && o.ld < (1L << 21)));
+    return left && left->format == NG_MX_FP4 && lines % 8 == 0 && o.ld % 8 == 0 && o.ld < (1L << 21);
 }
 
-static size_t pack_bytes(const ng_mx_operand& o, int lines, int k)
+// whether this product takes the kernel for few dense lines
+static bool is_skinny(const ng_mx_operand& A, const ng_mx_operand& B, int m, int n)
 {
-    if (o.format != NG_MX_NONE || dense_in_place(o, lines, k)) return 0;
+    return (A.format == NG_MX_FP4 && B.format == NG_MX_NONE && n <= 32) || (A.format == NG_MX_NONE && B.format == NG_MX_FP4 && m <= 32);
+}
+
+// room for a copy of a dense operand that is not laid out for its kernel
+static size_t pack_bytes(const ng_mx_operand& o, const ng_mx_operand* left, bool skinny, int lines, int k)
+{
+    if (o.format != NG_MX_NONE) return 0;
+    if (skinny && lines > 1) return mx_fragment_bytes(lines, k);
+    if (dense_in_place(o, skinny ? nullptr : left, lines, k)) return 0;
     return align_up((size_t)lines * padded_depth(k) * 2, 256);
 }
 
@@ -93,12 +87,9 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
     auto tiles = [&](int bm, int bn) { return (long)ceil_div(m, bm) * ceil_div(n, bn); };
     MxPlan p{128, 128, 64, 1, 0};
     int least = 4;
-    if (!is_44(A, B) && (A.format == NG_MX_FP4 || B.format == NG_MX_FP4)) {
-        const int dense_lines = A.format == NG_MX_NONE ? m : n;
-        if (dense_lines <= 32) {
-            p.skinny = (dense_lines + 15) / 16;
-            return p;
-        }
+    if (is_skinny(A, B, m, n)) {
+        p.skinny = ((A.format == NG_MX_NONE ? m : n) + 15) / 16;
+        return p;
     }
     if (is_44(A, B)) {
         p.bk = 256;
@@ -124,7 +115,7 @@ static MxSide make_side(const ng_mx_operand& o, int lines, int k)
     if (o.format == NG_MX_NONE) {
         s.pitch = o.ld * 2;
         s.scale_pitch = 0;
-        s.chunks = k / 8;
+        s.chunks = o.along ? k / 8 : k;     // rows, where the lines lie across them
         s.blocks = 0;
     } else {
         s.pitch = mx_code_pitch(o.format, k);
@@ -153,11 +144,9 @@ static void launch_tiles(const MxArgs& g, const MxPlan& p, const MxSide& a, cons
         else                  hipLaunchKernelGGL((mx44_kernel<64, 64, 256, 2, 2, 2, Epi>), grid, dim3(256), 0, g.stream, a, b, epi, s);
     } else {
         constexpr bool X_IS_A = FA != NG_MX_NONE;
-        constexpr int FMT = X_IS_A ? FA : FB;
         const MxSide &x = X_IS_A ? a : b, &d = X_IS_A ? b : a;
-        if (p.bm == 256) hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 256, 256, 4, 2, 3, Epi>), grid, dim3(512), 0, g.stream, x, d, epi, s);
-        else if (s.k_tiles <= 2) hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 128, 128, 2, 2, 2, Epi>), grid, dim3(256), 0, g.stream, x, d, epi, s);
-        else             hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, 128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, g.stream, x, d, epi, s);
+        const bool across = !(X_IS_A ? g.B : g.A).along;
+        launch_mix<X_IS_A ? FA : FB, Epi>(X_IS_A, across, p.bm, x, d, epi, s, grid, g.stream);
     }
 }
 
@@ -165,13 +154,15 @@ template <bool X_IS_A, class Epi>
 static int launch_skinny(const MxArgs& g, int groups, const MxSide& x, const MxSide& d, const Epi& epi)
 {
     const dim3 grid((unsigned)ceil_div(x.lines, 16));
-    // sixteen wavefronts keep more of a long line in flight
-    const bool deep = x.blocks >= 256;
-#define NG_SKINNY(NC, WAVES)                                                                                              \
-    hipLaunchKernelGGL((mx_skinny_kernel<X_IS_A, NC, WAVES, Epi>), grid, dim3(WAVES * 64), 0, g.stream, x, d, epi, x.lines, \
+    // as many wavefronts as the contraction has units of 256, up to what a workgroup (and
+    // with two groups of dense lines, the registers) holds: all loads of a short one are in flight at once
+    const int units = ceil_div(x.blocks, 8);
+#define NG_SKINNY(NC, WAVES, PACKED)                                                                                             \
+    hipLaunchKernelGGL((mx_skinny_kernel<X_IS_A, NC, WAVES, PACKED, Epi>), grid, dim3(WAVES * 64), 0, g.stream, x, d, epi, x.lines, \
                        d.lines, d.chunks)
-    if (groups == 1) { if (deep) NG_SKINNY(1, 16); else NG_SKINNY(1, 4); }
-    else             { if (deep) NG_SKINNY(2, 8); else NG_SKINNY(2, 4); }
+    if (d.lines == 1)     { if (units >= 16) NG_SKINNY(1, 16, false); else NG_SKINNY(1, 4, false); }
+    else if (groups == 1) { if (units >= 16) NG_SKINNY(1, 16, true); else NG_SKINNY(1, 4, true); }
+    else                  { if (units >= 16) NG_SKINNY(2, 8, true); else NG_SKINNY(2, 4, true); }
 #undef NG_SKINNY
     NG_CHECK_LAUNCH("mx product of few lines");
     return 0;
@@ -261,7 +252,8 @@ size_t ng_mx_gemm_workspace_bytes(int c_dtype, int m, int n, int k, const ng_mx_
     (void)c_dtype;
     const MxPlan p = choose_plan(m, n, k, *A, *B, SIZE_MAX);
     const size_t slices = p.splits > 1 ? align_up((size_t)p.splits * m * n * 4, 256) : 0;
-    return slices + pack_bytes(*A, m, k) + pack_bytes(*B, n, k);
+    const bool skinny = p.skinny != 0;
+    return slices + pack_bytes(*A, nullptr, skinny, m, k) + pack_bytes(*B, A, skinny, n, k);
 }
 
 int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const ng_mx_operand* B, void* C, int ldc,
@@ -275,25 +267,29 @@ int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const n
     if (ldc < n && m > 1) return fail(-101, "ng_mx_gemm: leading dimension of C smaller than row length");
     const size_t need = ng_mx_gemm_workspace_bytes(c_dtype, m, n, k, A, B);
     if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 15)))
-        return fail(-102, "ng_mx_gemm: this product needs %zu bytes of 16-byte aligned workspace, got %zu", need,
+        return fail(NG_MX_WORKSPACE, "ng_mx_gemm: this product needs %zu bytes of 16-byte aligned workspace, got %zu", need,
                     workspace ? workspace_bytes : (size_t)0);
     MxArgs g{c_dtype, m, n, k, *A, *B, C, ldc, alpha, beta, flags, seed, rng_stream,
              (char*)workspace, workspace_bytes, (hipStream_t)stream};
     // dense operands that are not laid out for the kernels are copied behind the slices
     char* end = g.ws + need;
     int lines = m;
+    const bool skinny = is_skinny(*A, *B, m, n);
     for (ng_mx_operand* o : {&g.A, &g.B}) {
-        const size_t bytes = pack_bytes(*o, lines, k);
-        if (bytes && k) {
+        const size_t bytes = k ? pack_bytes(*o, o == &g.B ? A : nullptr, skinny, lines, k) : 0;
+        if (bytes) {
             end -= bytes;
             const int padded = padded_depth(k);
             const unsigned short* from = (const unsigned short*)o->codes;
-            if (lines <= 64)
-                hipLaunchKernelGGL(mx_pack_few_kernel, dim3((unsigned)(((long)lines * (padded / 8) + 255) / 256)), dim3(256), 0, g.stream,
-                                   from, o->ld, o->along, lines, k, padded, (unsigned short*)end);
-            else
+            unsigned short* to = (unsigned short*)end;
+            if (skinny && lines > 1) {
+                const unsigned total = (unsigned)(bytes / 16);
+                hipLaunchKernelGGL(mx_pack_fragments_kernel, dim3((total + 255u) / 256u), dim3(256), 0, g.stream, from, o->ld, o->along,
+                                   lines, k, (lines + 15) / 16, total, to);
+            } else {
                 hipLaunchKernelGGL(mx_pack_kernel, dim3((unsigned)ceil_div(lines, 64), (unsigned)ceil_div(padded, 64)), dim3(256), 0,
-                                   g.stream, from, o->ld, o->along, lines, k, padded, (unsigned short*)end);
+                                   g.stream, from, o->ld, o->along, lines, k, padded, to);
+            }
             NG_CHECK_LAUNCH("mx pack");
             o->codes = end;
             o->along = 1;
@@ -303,8 +299,8 @@ int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const n
     }
     g.ws_bytes = (size_t)(end - g.ws);
     const int kd = (g.A.format == NG_MX_NONE || g.B.format == NG_MX_NONE) ? padded_depth(k) : k;
-    const MxSide a = make_side(g.A, m, g.A.format == NG_MX_NONE ? kd : k);
-    const MxSide b = make_side(g.B, n, g.B.format == NG_MX_NONE ? kd : k);
+    const MxSide a = make_side(g.A, m, g.A.format == NG_MX_NONE && g.A.along ? kd : k);
+    const MxSide b = make_side(g.B, n, g.B.format == NG_MX_NONE && g.B.along ? kd : k);
     return c_dtype == NG_F16 ? dispatch<_Float16>(g, a, b) : dispatch<float>(g, a, b);
 }
 

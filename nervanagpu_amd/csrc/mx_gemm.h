@@ -104,6 +104,52 @@ struct MxFetch {
     }
 };
 
+// A dense operand whose lines lie across the contiguous axis (value i of line r at
+// [i * ld + r]): 64 rows of LINES neighbouring values, read with the transposing LDS
+// read, which takes 64 bytes from each of 4 rows, so rows differ in their 64-byte group.
+template <int LINES>
+struct MxAcrossTile {
+    static constexpr int CPR = LINES / 8;
+    static constexpr int PITCH = LINES * 2;
+    static constexpr int CHUNKS = 64 * CPR;
+    static constexpr int BYTES = 64 * PITCH;
+    static_assert(CPR % 16 == 0, "the swizzle permutes four groups of 64 bytes");
+    static __device__ __forceinline__ int swizzle(int i) { return (i & 3) * 4; }
+};
+
+template <class Tile, int NT>
+struct MxAcrossFetch {
+    static constexpr int DATA = Tile::CHUNKS / NT, STEP = NT / Tile::CPR;
+    static_assert(Tile::CHUNKS % NT == 0 && NT % Tile::CPR == 0 && STEP % 4 == 0, "requests must be whole periods of the swizzle");
+    const char* base;        // of the next tile
+    int pitch, row_bytes;    // of a row of the matrix; from this tile's first line to the last one
+    int left;                // rows not yet fetched
+    unsigned off;
+    // s.lines: lines (values of a row), s.chunks: rows
+    __device__ __forceinline__ void init(const MxSide& s, int line0, int kt, int tid)
+    {
+        pitch = (int)s.pitch;
+        row_bytes = min(s.lines - line0, Tile::CPR * 8) * 2;
+        base = s.data + (long)kt * 64 * s.pitch + (long)line0 * 2;
+        left = s.chunks - kt * 64;
+        const int i = tid / Tile::CPR, c = (tid % Tile::CPR) ^ Tile::swizzle(i);
+        off = c * 16 < row_bytes ? (unsigned)i * (unsigned)pitch + (unsigned)c * 16u : NG_OOB_OFFSET;
+    }
+    __device__ __forceinline__ unsigned lane_offset() const { return off; }
+    __device__ __forceinline__ void issue(int i, unsigned lane_off, char* lds, int wave) const
+    {
+        const int rows = min(left - i * STEP, STEP);
+        const BufferRsrc r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(base + (long)(i * STEP) * pitch), 0,
+                                                               rows > 0 ? (rows - 1) * pitch + row_bytes : 0, 0x00020000);
+        buffer_load_chunk_to_lds(r, lds + (i * NT + wave * 64) * 16, lane_off);
+    }
+    __device__ __forceinline__ void advance()
+    {
+        base += 64l * pitch;
+        left -= 64;
+    }
+};
+
 // Scale of an int8 block as fp16 factors.  code * 2^e is formed as
 // ((1024 + code + 128) * s1 - 1152 * s1) * s2 with s1 s2 = 2^e: the bytes become
 // fp16 1024 + u by placing them under the exponent of 1024, s1 = 2^(-14 .. 5) keeps
@@ -411,8 +457,9 @@ template <> struct MxBlock<NG_MX_INT8> {
 
 // X: the block-scaled operand (rows of C if X_IS_A, else its columns), D: the dense one.
 // WX x WD wavefronts; a wavefront expands BX / WX lines of codes and multiplies them
-// with BD / WD dense lines, so few X lines a wavefront mean little expansion.
-template <int FMT, bool X_IS_A, int BX, int BD, int WX, int WD, int NSTAGE, class Epi>
+// with BD / WD dense lines, so few X lines a wavefront mean little expansion.  ACROSS: the
+// dense lines lie across the contiguous axis.
+template <int FMT, bool X_IS_A, bool ACROSS, int BX, int BD, int WX, int WD, int NSTAGE, class Epi>
 __global__ __launch_bounds__(WX * WD * 64)
 void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
 {
@@ -422,9 +469,9 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     constexpr int TM = X_IS_A ? TX : TD, TN = X_IS_A ? TD : TX, WTN = TN * 32;
     using Block = MxBlock<FMT>;
     using TileX = MxTile<BX, 2 * Block::BYTES>;
-    using TileD = MxTile<BD, 128>;
+    using TileD = std::conditional_t<ACROSS, MxAcrossTile<ACROSS ? BD : 128>, MxTile<BD, 128>>;
     using FX = MxFetch<TileX, NT>;
-    using FD = MxFetch<TileD, NT>;
+    using FD = std::conditional_t<ACROSS, MxAcrossFetch<MxAcrossTile<ACROSS ? BD : 128>, NT>, MxFetch<MxTile<BD, 128>, NT>>;
     // scales: groups of 16 blocks (8 tiles), four lanes a line, in a ring of two slots
     constexpr int SPER = BX / 16 / WAVES, SLOT = BX * 16;
     static_assert(BX % (16 * WAVES) == 0 && SPER <= 4, "scale requests must divide evenly over wavefronts");
@@ -486,7 +533,21 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     constexpr int XC = Block::BYTES / 16;             // chunks of a block
     const int x_off = TileX::offset(wx * TX * 32 + row, half * XC);
     const int x_second = XC == 2 ? TileX::offset(row, half * XC + 1) - TileX::offset(row, half * XC) : 0;
-    const int d_off = TileX::BYTES + TileD::offset(wd * TD * 32 + row, half * 4);
+    // dense fragments: contiguous lines have one address (the swizzle only depends on the
+    // line inside a block of 32); lines across have one per block of 32, of row 32 half + (l / 4)
+    // and the lane's 8-byte piece (l: lane inside 16)
+    constexpr int DOFF = ACROSS ? TD : 1;
+    int d_off[DOFF];
+    if constexpr (ACROSS) {
+        const int l = lane & 15, i = half * 32 + (l >> 2);
+#pragma unroll
+        for (int t = 0; t < TD; t++) {
+            const int c = (wd * TD + t) * 4 + ((lane >> 4) & 1) * 2 + ((l >> 1) & 1);
+            d_off[t] = TileX::BYTES + i * TileD::PITCH + ((c ^ TileD::swizzle(i)) * 16) + (l & 1) * 8;
+        }
+    } else {
+        d_off[0] = TileX::BYTES + TileD::offset(wd * TD * 32 + row, half * 4);
+    }
     const int s_read = SCALES + (wx * TX * 32 + row) * 16 + half;
 
     Block blk[TX];
@@ -499,7 +560,15 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     };
     // dense chunk 4 half + step of the line: the xor with the swizzle distributes
     auto load_dense = [&](int stage_off, int step, int to, int i) {
-        fd_[to][i] = *reinterpret_cast<const half8_t*>(smem + stage_off + (d_off ^ (step * 16)) + i * 32 * 128);
+        if constexpr (ACROSS) {
+            const char* p = smem + stage_off + d_off[ACROSS ? i : 0] + step * 8 * TileD::PITCH;
+            const short4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NG_LDS short4_t*)(p));
+            const short4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((NG_LDS short4_t*)(p + 4 * TileD::PITCH));
+            const short8_t both = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            fd_[to][i] = __builtin_bit_cast(half8_t, both);
+        } else {
+            fd_[to][i] = *reinterpret_cast<const half8_t*>(smem + stage_off + (d_off[0] ^ (step * 16)) + i * 32 * 128);
+        }
     };
     auto product = [&](int step, int p) {
         const int i = p / TN, j = p % TN;
@@ -592,5 +661,10 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     const int wm = X_IS_A ? wx : wd, wn = X_IS_A ? wd : wx;
     EpilogueBands<TM, TN, WTN, EPITCH, 0>::run(acc, stage, lane, m0 + wm * TM * 32, n0 + wn * WTN, 0, split, epi);
 }
+
+// tile: 256 or 128 lines of either side; defined in mx_mix.hip for the epilogues of products
+template <int FMT, class Epi>
+void launch_mix(bool x_is_a, bool across, int tile, const MxSide& x, const MxSide& d, const Epi& epi, const CoreShape& s, dim3 grid,
+                hipStream_t stream);
 
 }  // namespace ng

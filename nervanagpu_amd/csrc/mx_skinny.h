@@ -12,12 +12,42 @@
 
 namespace ng {
 
-// NC: groups of 16 dense lines
-template <bool X_IS_A, int NC, int WAVES, class Epi>
+// Dense lines in fragment order: of every 256 values, 8 requests of a wavefront (16 bytes
+// a lane, contiguous), request p holding for lane l values 128 (p / 4) + 32 (l / 16) + 8 (p % 4) .. + 7
+// of line 16 c + l % 16; zeros where the matrix ends.  Read where they lie, 64 lanes' pieces
+// would be 64 requests: 25088 x 16 values took 24 us of a 33 us product.
+constexpr int MX_SKINNY_UNIT = 256;
+inline size_t mx_fragment_bytes(int lines, int k)
+{
+    return (size_t)((k + MX_SKINNY_UNIT - 1) / MX_SKINNY_UNIT) * ((lines + 15) / 16) * 8192;
+}
+
+static __global__ __launch_bounds__(256)
+void mx_pack_fragments_kernel(const unsigned short* __restrict__ X, long ld, int along, int lines, int depth, int groups,
+                              unsigned total, unsigned short* __restrict__ out)
+{
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;      // ((unit * groups + c) * 8 + p) * 64 + lane
+    if (id >= total) return;
+    const int lane = (int)(id & 63u), p = (int)((id >> 6) & 7u);
+    const int uc = (int)(id >> 9), u = uc / groups, c = uc - u * groups;
+    const int line = c * 16 + (lane & 15), k0 = u * MX_SKINNY_UNIT + (p >> 2) * 128 + (lane >> 4) * 32 + (p & 3) * 8;
+    unsigned short v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++)
+        v[i] = (line < lines && k0 + i < depth) ? X[along ? (long)line * ld + k0 + i : (long)(k0 + i) * ld + line] : (unsigned short)0;
+    uint4_t w;
+    __builtin_memcpy(&w, v, 16);
+    *reinterpret_cast<uint4_t*>(out + (size_t)id * 8) = w;
+}
+
+// NC: groups of 16 dense lines; PACKED: they are in fragment order, else one line lies
+// contiguous (and the lanes of the others read nothing)
+template <bool X_IS_A, int NC, int WAVES, bool PACKED, class Epi>
 __global__ __launch_bounds__(WAVES * 64)
 void mx_skinny_kernel(MxSide x, MxSide d, Epi epi, int xl, int dl, int depth8)
 {
-    constexpr int UNIT = 256;               // values an iteration takes: two blocks a lane, 8 bytes of scales a line
+    constexpr int UNIT = MX_SKINNY_UNIT;    // values an iteration takes: two blocks a lane, 8 bytes of scales a line
+    static_assert(PACKED || NC == 1, "only a single line is read where it lies");
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int row = lane & 15, quarter = lane >> 4;
@@ -29,9 +59,7 @@ void mx_skinny_kernel(MxSide x, MxSide d, Epi epi, int xl, int dl, int depth8)
     // lines past the end read line 0 and are not stored
     const char* codes = x.data + (long)(x0 + row < xl ? x0 + row : x0) * x.pitch + quarter * 16;
     const char* scales = x.scales + (long)(x0 + row < xl ? x0 + row : x0) * x.scale_pitch;
-    const char* dense[NC];
-#pragma unroll
-    for (int c = 0; c < NC; c++) dense[c] = d.data + (long)min(c * 16 + row, dl - 1) * d.pitch + quarter * 64;
+    const char* dense = PACKED ? d.data + lane * 16 : d.data + quarter * 64;
 
     struct Stage { uint4_t q[2]; uint2v_t s; half8_t v[NC][8]; };
     auto fetch = [&](int u, Stage& st) {
@@ -46,9 +74,13 @@ void mx_skinny_kernel(MxSide x, MxSide d, Epi epi, int xl, int dl, int depth8)
         for (int c = 0; c < NC; c++)
 #pragma unroll
             for (int p = 0; p < 8; p++) {
-                const int k8 = u * (UNIT / 8) + (p >> 2) * 16 + quarter * 4 + (p & 3);     // which 8 values
-                st.v[c][p] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
-                if (k8 < depth8) st.v[c][p] = *reinterpret_cast<const half8_t*>(dense[c] + (long)u * (UNIT * 2) + (p >> 2) * 256 + (p & 3) * 16);
+                if constexpr (PACKED) {
+                    st.v[c][p] = *reinterpret_cast<const half8_t*>(dense + ((long)u * NC + c) * 8192 + p * 1024);
+                } else {
+                    const int k8 = u * (UNIT / 8) + (p >> 2) * 16 + quarter * 4 + (p & 3);     // which 8 values
+                    st.v[c][p] = half8_t{0, 0, 0, 0, 0, 0, 0, 0};
+                    if (k8 < depth8 && row == 0) st.v[c][p] = *reinterpret_cast<const half8_t*>(dense + (long)u * (UNIT * 2) + (p >> 2) * 256 + (p & 3) * 16);
+                }
             }
     };
     float4_t acc[NC];

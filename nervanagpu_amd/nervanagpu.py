@@ -25,6 +25,7 @@ _DTYPE_CODE = {np.dtype(np.float16): _lib.NG_F16, np.dtype(np.float32): _lib.NG_
                np.dtype(np.uint8): _lib.NG_U8, np.dtype(np.int8): _lib.NG_I8}
 
 
+_FLOATS = (np.float16, np.float32)
 _ACT_CODE = {"relu": 0, "sig": 1, "tanh": 2, "silu": 3, "gelu": 4}
 
 
@@ -695,24 +696,33 @@ class NervanaGPU(object):
         """a host matrix converted to a block-scaled one"""
         return self.mx_empty(ary.shape, fmt, axis, name, rounding).set(ary)
 
-    def _mx_dense(self, A, axis, what):
+    @staticmethod
+    def _mx_dense(A, axis, what):
         """(pitch, whether lines along `axis` are contiguous) of a dense 2-D tensor"""
-        assert isinstance(A, GPUTensor) and len(A.shape) == 2 and not A.take_array, "%s must be a 2-D tensor" % what
-        if not A.size:
-            return A.shape[axis], 1
-        assert min(A.strides) >= 1 and (1 in A.strides), "one dimension of %s must be contiguous" % what
-        if A.strides[axis] == 1 and (A.strides[1 - axis] >= A.shape[axis] or A.shape[1 - axis] <= 1):
-            return A.strides[1 - axis], 1
-        assert A.strides[1 - axis] == 1, "one dimension of %s must be contiguous" % what
-        return A.strides[axis], 0
+        shape, strides = A.shape, A.strides
+        assert len(shape) == 2 and not A.take_array, "%s must be a 2-D tensor" % what
+        inner, outer = strides[axis], strides[1 - axis]
+        depth, lines = shape[axis], shape[1 - axis]
+        if inner == 1:
+            if outer >= depth:
+                return outer, 1
+            if lines <= 1:
+                return depth, 1
+        if outer == 1:
+            if inner >= lines:
+                return inner, 0
+            if depth <= 1:
+                return lines, 0
+        assert not A.size, "one dimension of %s must be contiguous" % what
+        return depth, 1
 
     def mx_quantize(self, A, out, repeat=1):
         """out = A in blocks of 32 values that share a power of two.  A: fp16 or fp32
         matrix with one contiguous dimension.  Rounds to the nearest code (ties to
         even), or stochastically if out.rounding is set: then every value is right on
         average.  A block with an infinity or a NaN becomes NaN.  Returns out."""
-        assert isinstance(out, MXTensor) and A.shape == out.shape
-        if A.dtype.type not in (np.float16, np.float32):
+        assert type(out) is MXTensor and A.shape == out.shape
+        if A.dtype.type not in _FLOATS:
             raise TypeError("Only floating point tensors can be quantized.")
         ld, along = self._mx_dense(A, out.axis, "A")
         if not out.size:
@@ -725,8 +735,8 @@ class NervanaGPU(object):
 
     def mx_dequantize(self, A, out):
         """out (fp16 or fp32) = the values of the block-scaled A; returns out"""
-        assert isinstance(A, MXTensor) and A.shape == out.shape
-        if out.dtype.type not in (np.float16, np.float32):
+        assert type(A) is MXTensor and A.shape == out.shape
+        if out.dtype.type not in _FLOATS:
             raise TypeError("Only floating point tensors can be dequantized into.")
         ld, along = self._mx_dense(out, A.axis, "out")
         if A.size:
@@ -736,7 +746,7 @@ class NervanaGPU(object):
 
     def _mx_side(self, X, axis, what):
         """an operand of mx_dot whose contraction is its axis `axis`"""
-        if isinstance(X, MXTensor):
+        if type(X) is MXTensor:
             if X.axis != axis:
                 raise ValueError("the blocks of %s must run along the contraction (axis %d)" % (what, axis))
             return X.operand()
@@ -753,35 +763,37 @@ class NervanaGPU(object):
         taken as fp16).  Blocks run along k: A has axis 1, B has axis 0.
         C: fp16 or fp32, rows or columns contiguous; stochastic rounding as in dot.
         """
-        if not isinstance(A, MXTensor) and not isinstance(B, MXTensor):
+        if type(A) is MXTensor:
+            if type(B) is MXTensor and not A.fmt == B.fmt == "fp4":
+                raise TypeError("block-scaled operands must both be fp4, or one operand a dense fp16 tensor")
+        elif type(B) is not MXTensor:
             raise TypeError("mx_dot needs a block-scaled operand (dot multiplies dense ones)")
-        if isinstance(A, MXTensor) and isinstance(B, MXTensor) and (A.fmt, B.fmt) != ("fp4", "fp4"):
-            raise TypeError("block-scaled operands must both be fp4, or one operand a dense fp16 tensor")
-        if C.dtype.type not in (np.float16, np.float32):
+        if C.dtype.type not in _FLOATS:
             raise TypeError("Only floating point dot currently supported.")
+        a, b = self._mx_side(A, 1, "A"), self._mx_side(B, 0, "B")
         (m, k), n = A.shape, B.shape[1]
         assert C.shape == (m, n) and B.shape[0] == k
-        assert len(C.strides) == 2 and not C.take_array
-        a, b = self._mx_side(A, 1, "A"), self._mx_side(B, 0, "B")
         ldc, by_rows = self._mx_dense(C, 1, "C")
         if not by_rows:
             # columns contiguous: the transposed product
             m, n, a, b = n, m, b, a
-        code = _DTYPE_CODE[C.dtype]
-        flags = 0
-        if C.rounding:
-            flags |= 1 | (int(C.rounding) << 16)
-        if relu:
-            flags |= 2
         if not C.size:
             return C
-        need = _lib.load().ng_mx_gemm_workspace_bytes(code, m, n, k, a, b)
-        ws, ws_bytes = self._get_scratch(need)
-        stream = self.stream
+        code = _DTYPE_CODE[C.dtype]
+        rounding = C.rounding
+        flags = (1 | (int(rounding) << 16) if rounding else 0) | (2 if relu else 0)
+        stream, c_ptr, gemm = self.stream, C.ptr, _lib.load().ng_mx_gemm
 
         def launch():
-            seed, sid = self._next_rng_stream() if C.rounding else (0, 0)
-            _lib.call("ng_mx_gemm", code, m, n, k, a, b, C.ptr, ldc, alpha, beta, flags, seed, sid, int(ws), ws_bytes, stream)
+            seed, sid = self._next_rng_stream() if rounding else (0, 0)
+            ws, ws_bytes = self._get_scratch(0)
+            status = gemm(code, m, n, k, a, b, c_ptr, ldc, alpha, beta, flags, seed, sid, int(ws), ws_bytes, stream)
+            if status == _lib.NG_MX_WORKSPACE:
+                # nothing has been launched: the arena grows and the call is made again
+                ws, ws_bytes = self._get_scratch(_lib.load().ng_mx_gemm_workspace_bytes(code, m, n, k, a, b))
+                status = gemm(code, m, n, k, a, b, c_ptr, ldc, alpha, beta, flags, seed, sid, int(ws), ws_bytes, stream)
+            if status:
+                _lib.check(status)
 
         if repeat > 1:
             for r in range(max(repeat // 10, 1)):
@@ -801,19 +813,29 @@ class NervanaGPU(object):
                 return gflops
         return C
 
-    def _act_operand(self, X, like, what):
-        """row pitch of an operand of an activation function"""
-        if X.dtype.type not in (np.float16, np.float32):
+    def _act_operands(self, op, dense, saved):
+        """(op code, dtype code, rows, cols, codes, scales, pitches) of an activation
+        function's operands, all checked"""
+        code = _ACT_CODE.get(op)
+        if code is None:
+            raise ValueError("unknown activation function %r (%s)" % (op, ", ".join(sorted(_ACT_CODE))))
+        first = dense[0]
+        if first.dtype.type not in _FLOATS:
             raise TypeError("Only floating point activations are supported.")
-        assert X.shape == like.shape and X.dtype == like.dtype, "%s must match the other operands" % what
-        ld, along = self._mx_dense(X, 1, what)
-        assert along, "rows of %s must be contiguous" % what
-        return ld
-
-    def _act_saved(self, saved, shape):
-        assert isinstance(saved, MXTensor) and saved.shape == tuple(shape)
-        if saved.fmt != "int8" or saved.axis != 1 or saved.rounding:
-            raise ValueError("a checkpoint of activations is an int8 MXTensor with axis 1 and nearest rounding")
+        lds = []
+        for X in dense:
+            assert X.shape == first.shape and X.dtype == first.dtype, "activation operands must match"
+            ld, along = self._mx_dense(X, 1, "an activation operand")
+            assert along, "rows of activation operands must be contiguous"
+            lds.append(ld)
+        codes = scales = None
+        if saved is not None:
+            assert type(saved) is MXTensor and saved.shape == first.shape, "the checkpoint must match the operands"
+            if saved.fmt != "int8" or saved.axis != 1 or saved.rounding:
+                raise ValueError("a checkpoint of activations is an int8 MXTensor with axis 1 and nearest rounding")
+            if saved.size:
+                codes, scales = saved.codes.ptr, saved.scales.ptr
+        return code, _DTYPE_CODE[first.dtype], first.shape[0], first.shape[1], codes, scales, lds
 
     def fprop_act(self, op, I, O, saved=None):
         """
@@ -822,26 +844,18 @@ class NervanaGPU(object):
         op: "relu", "sig", "tanh", "silu" (x sig(x)) or "gelu" (x times the normal
         distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous
         """
-        if op not in _ACT_CODE:
-            raise ValueError("unknown activation function %r (%s)" % (op, ", ".join(sorted(_ACT_CODE))))
-        ldi, ldo = self._act_operand(I, I, "I"), self._act_operand(O, I, "O")
-        if saved is not None:
-            self._act_saved(saved, I.shape)
+        code, dtype, rows, cols, codes, scales, (ldi, ldo) = self._act_operands(op, (I, O), saved)
         if I.size:
-            _lib.call("ng_act_fprop", _ACT_CODE[op], _DTYPE_CODE[I.dtype], I.shape[0], I.shape[1], I.ptr, ldi, O.ptr, ldo,
-                      saved.codes.ptr if saved is not None else None, saved.scales.ptr if saved is not None else None, self.stream)
+            _lib.call("ng_act_fprop", code, dtype, rows, cols, I.ptr, ldi, O.ptr, ldo, codes, scales, self.stream)
         return O
 
     def bprop_act(self, op, saved, E, grad_I):
         """grad_I = E * op'(saved): the derivative is taken at the values the 8-bit
         checkpoint of fprop_act stands for.  grad_I may be E."""
-        if op not in _ACT_CODE:
-            raise ValueError("unknown activation function %r (%s)" % (op, ", ".join(sorted(_ACT_CODE))))
-        lde, ldg = self._act_operand(E, E, "E"), self._act_operand(grad_I, E, "grad_I")
-        self._act_saved(saved, E.shape)
+        assert saved is not None, "bprop_act needs the checkpoint of fprop_act"
+        code, dtype, rows, cols, codes, scales, (lde, ldg) = self._act_operands(op, (E, grad_I), saved)
         if E.size:
-            _lib.call("ng_act_bprop", _ACT_CODE[op], _DTYPE_CODE[E.dtype], E.shape[0], E.shape[1], saved.codes.ptr,
-                      saved.scales.ptr, E.ptr, lde, grad_I.ptr, ldg, self.stream)
+            _lib.call("ng_act_bprop", code, dtype, rows, cols, codes, scales, E.ptr, lde, grad_I.ptr, ldg, self.stream)
         return grad_I
 
     def compensated_sum(self, sum_tensor, cmp_tensor, add_tensor, cmp_scale=1.0, add_scale=1.0):

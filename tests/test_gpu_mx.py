@@ -183,7 +183,7 @@ def test_fp4_product(ng, m, n, k, out):
 
 
 @pytest.mark.parametrize("kinds", ["44", "4h", "h4", "8h", "h8"])
-@pytest.mark.parametrize("m,n,k", [(530, 1030, 1100), (2900, 3080, 300)])
+@pytest.mark.parametrize("m,n,k", [(520, 264, 264), (530, 1030, 1100), (2900, 3080, 300)])
 def test_larger_products(ng, kinds, m, n, k):
     """several tiles in both directions, ragged; the second fills the chip"""
     rng = np.random.default_rng(k)
