@@ -260,7 +260,7 @@ int ng_mx_dequantize(int format, const void* codes, const void* scales, int line
 
 /* Activation function of a (rows, cols) matrix with an 8-bit checkpoint of its
  * input for the backward pass (NG_MX_INT8, a line per row).
- *   ng_act_fprop  O = f(I); codes and scales, unless NULL, receive I
+ *   ng_act_fprop  O = f(I); codes and scales, unless NULL, receive I; O may be I
  *   ng_act_bprop  gradI = E * f'(the values of the checkpoint); gradI may be E
  * E, O and gradI have the dtype (NG_F16 or NG_F32) of I; ldi, ldo, lde, ldg are row
  * pitches in elements. */

@@ -116,8 +116,9 @@ def _inception(kind, w):
     return {"layer": Inception, "partitions": tuple(parts)}
 
 
-def network_config(name):
-    """list of Layer.create configuration dicts for a named network"""
+def network_config(name, fc_options=None):
+    """list of Layer.create configuration dicts for a named network; fc_options:
+    further keys of the dense layers (mx4, save8)"""
     net = _NETS[name]
     confs = [{"layer": DataLayer, "N": net["N"], "C": 3, "H": net["H"], "W": net["H"]}]
     for spec in net["layers"]:
@@ -128,7 +129,7 @@ def network_config(name):
         elif spec[0] in ("incep1", "incep2"):
             confs.append(_inception(*spec))
         else:
-            confs.append({"layer": FullLayer, "nOut": spec[1]})
+            confs.append(dict(fc_options or {}, layer=FullLayer, nOut=spec[1]))
     return confs
 
 
@@ -137,11 +138,17 @@ def fold_relu_derivatives(layers):
     connected layer's rectifier derivative, so that layer skips its elementwise
     pass over the errors.  A max pooling layer above reads the same activations
     to find its maxima (no extra traffic); a unit-stride convolution above
-    reads them once in its store.  Same results; not part of the reference's
+    reads them once in its store; a dense layer above that keeps its input in
+    8 bits reads those (where they round an activation to zero its derivative is
+    zero too).  Otherwise the same results; not part of the reference's
     driver.  Returns the number of folded pairs."""
     folded = 0
     for below, above in zip(layers[:-1], layers[1:]):
         if type(below) not in (ConvLayer, FullLayer):
+            continue
+        if type(above) is FullLayer and above.save8:
+            above.relu_below = below.relu_done_above = True
+            folded += 1
             continue
         if type(above) is PoolLayer and above.op == "max" and reduce(mul, above.JTRS, 1) <= 255:
             above.relu_below = True
@@ -196,9 +203,10 @@ def build_network(ng, confs, dtype, zeros=False, seed=0, fold_relu=False):
     return layers
 
 
-def run_network(ng, name, dtype, loops=10, zeros=False, verbose=True, out=sys.stdout, fold_relu=False, warmup=None):
+def run_network(ng, name, dtype, loops=10, zeros=False, verbose=True, out=sys.stdout, fold_relu=False, warmup=None,
+                fc_options=None):
     net = _NETS[name]
-    layers = build_network(ng, network_config(name), dtype, zeros=zeros, fold_relu=fold_relu)
+    layers = build_network(ng, network_config(name, fc_options), dtype, zeros=zeros, fold_relu=fold_relu)
     start, end = _lib.Event(), _lib.Event()
     # untimed iterations: the reference's count unless the caller asks for more (sustained clocks)
     warmup = net["warmup"] if warmup is None else max(int(warmup), net["warmup"])
@@ -261,7 +269,14 @@ def main(argv=None):
                     help="let max pooling and unit-stride convolution backward apply the rectifier derivative of "
                          "the layer below them (same results, one elementwise pass per such pair saved; not in "
                          "the reference)")
+    ap.add_argument("--fc-mx4", action="store_true",
+                    help="fp16 networks: dense layers multiply 4-bit block-scaled copies of weights, inputs and errors")
+    ap.add_argument("--fc-save8", action="store_true",
+                    help="fp16 networks: dense layers keep their input for the backward pass in 8 bits")
     args = ap.parse_args(argv)
+    fc_options = {k: True for k, on in (("mx4", args.fc_mx4), ("save8", args.fc_save8)) if on}
+    if fc_options and args.dtypes != "f16":
+        ap.error("--fc-mx4 and --fc-save8 need --dtypes f16")
     dtypes = {"f16": np.float16, "f32": np.float32}
     ng = NervanaGPU(stochastic_round=False, bench=False)
     results = []
@@ -272,7 +287,7 @@ def main(argv=None):
             print("Benchmarking: " + title)
             print("------------------------------------------------")
             r = run_network(ng, name, dtypes[d], loops=args.loops, zeros=args.zeros, verbose=not args.quiet, warmup=args.warmup,
-                            fold_relu=args.fold_relu)
+                            fold_relu=args.fold_relu, fc_options=fc_options)
             results.append(r)
             print("---------------------------------------------")
             print(title + " Results:")

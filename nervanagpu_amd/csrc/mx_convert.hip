@@ -283,7 +283,7 @@ NG_DEV float act_slope(float z)
 
 template <typename T, int ACT, bool SAVE, bool VEC>
 __global__ __launch_bounds__(256)
-void act_fprop_kernel(const T* __restrict__ I, long ldi, T* __restrict__ O, long ldo, UnitMap map,
+void act_fprop_kernel(const T* I, long ldi, T* O, long ldo, UnitMap map,
                       unsigned char* __restrict__ codes, unsigned char* __restrict__ scales, long scale_pitch)
 {
     const unsigned u = blockIdx.x * 256u + threadIdx.x;

@@ -251,9 +251,22 @@ class DataLayer(Layer):
 
 class FullLayer(Layer):
     """Dense layer on (features, N) matrices: three GEMMs per training step
-    (nervanagpu/layers.py:254-273)."""
+    (nervanagpu/layers.py:254-273).
 
-    def __init__(self, lib, dtype, N, nIn, nOut):
+    Not in the reference, fp16 layers only, off by default:
+
+    mx4     y = W x and dx = W^T e multiply 4-bit block-scaled copies of W, x and e
+            (blocks along the contraction of each product, made in every step; they
+            round stochastically if the backend does).  The weights themselves and
+            their gradient stay as they are.
+    save8   the input is kept for the backward pass in 8 bits (saved_in): the weight
+            gradient, and with relu_below the rectifier derivative of the layer
+            below, are computed from what those stand for.  The fp16 input may be
+            overwritten once fprop has returned, so layers may share activation
+            buffers (init_activations(shared=...)).
+    """
+
+    def __init__(self, lib, dtype, N, nIn, nOut, mx4=False, save8=False):
         super(FullLayer, self).__init__(lib, dtype, N)
         self.nIn, self.nOut = nIn, nOut
         self.dimI = self.dimI2 = (nIn, N)
@@ -261,17 +274,55 @@ class FullLayer(Layer):
         self.dimF = self.dimF2 = (nOut, nIn)
         self.sizeI, self.sizeO, self.sizeF = nIn * N, nOut * N, nIn * nOut
         self.flops = N * nIn * nOut * 2.0
+        if mx4 or save8:
+            assert np.dtype(dtype).type is np.float16, "block-scaled layers are fp16 layers"
+        self.mx4, self.save8 = mx4, save8
+        self.relu_below = False         # with save8: apply (input > 0) to the error passed down
+        self.saved_in = None
+        self._mx = {}
+
+    def _mx_copy(self, name, source, axis):
+        """the 4-bit copy of `source` for one product, in a tensor kept for it"""
+        if name not in self._mx:
+            self._mx[name] = self.lib.mx_empty(source.shape, "fp4", axis)
+        return self.lib.mx_quantize(source, self._mx[name])
+
+    def init_activations(self, shared=None):
+        """own output buffer, or a view of shared[0]; the list is then flipped, as
+        in init_deltas.  Sharing needs save8 on every layer that reads a shared
+        buffer, and relu_below there (the rectifier of an overwritten output is
+        known from its 8-bit copy alone)."""
+        if shared is None:
+            return super(FullLayer, self).init_activations()
+        self.fprop_out = shared[0].share(self.dimO)
+        self.act_stats = self._stat_buffer(self.dimO2)
+        shared.reverse()
 
     def fprop(self, fprop_in, scale_weights=0):
         x = super(FullLayer, self).fprop(fprop_in)
-        self.lib.dot(self.weights, x, self.fprop_out, relu=True)            # y = relu(W x)
+        if self.mx4:
+            self.lib.mx_dot(self._mx_copy("W", self.weights, 1), self._mx_copy("x", x, 0), self.fprop_out, relu=True)
+        else:
+            self.lib.dot(self.weights, x, self.fprop_out, relu=True)        # y = relu(W x)
+        if self.save8:
+            if self.saved_in is None:
+                self.saved_in = self.lib.mx_empty(self.dimI, "int8", 1, rounding=0)
+            self.lib.mx_quantize(x, self.saved_in)
         self._rerun_scaled(x, scale_weights)
         return self.fprop_out
 
     def bprop(self, bprop_in):
         err = self.bprop_relu(bprop_in)
-        self.lib.dot(self.weights.T, err, self.bprop_out)                   # dx = W^T e
-        self.lib.dot(err, self.fprop_in.T, self.updat_out)                  # dW = e x^T
+        if self.mx4:
+            self.lib.mx_dot(self._mx_copy("W^T", self.weights, 0).T, self._mx_copy("e", err, 0), self.bprop_out)
+        else:
+            self.lib.dot(self.weights.T, err, self.bprop_out)               # dx = W^T e
+        if self.save8:
+            self.lib.mx_dot(err, self.saved_in.T, self.updat_out)
+            if self.relu_below:
+                self.lib.bprop_act("relu", self.saved_in, self.bprop_out, self.bprop_out)
+        else:
+            self.lib.dot(err, self.fprop_in.T, self.updat_out)              # dW = e x^T
         self.grad_descent()
         return self.bprop_out
 

@@ -842,7 +842,7 @@ class NervanaGPU(object):
         O = op(I), and saved (an MXTensor, fmt "int8", axis 1) = I, in one pass.
 
         op: "relu", "sig", "tanh", "silu" (x sig(x)) or "gelu" (x times the normal
-        distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous
+        distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous; O may be I
         """
         code, dtype, rows, cols, codes, scales, (ldi, ldo) = self._act_operands(op, (I, O), saved)
         if I.size:

@@ -408,6 +408,9 @@ def test_activation_and_checkpoint(ng, op, shape, dtype):
     compare(Y.get(), ref, tol)
     Y2 = ng.empty(shape, dtype=dtype)
     assert np.array_equal(ng.fprop_act(op, dZ, Y2).get(), Y.get())     # without a checkpoint
+    Q2, Z2 = ng.mx_empty(shape, "int8"), ng.array(z, dtype=dtype)
+    assert np.array_equal(ng.fprop_act(op, Z2, Z2, saved=Q2).get(), Y.get())   # in place
+    assert np.array_equal(Q2.codes.get(), Q.codes.get()) and np.array_equal(Q2.get(), Q.get())
     e = rng.standard_normal(shape).astype(dtype)
     G = ng.array(e, dtype=dtype)
     ng.bprop_act(op, Q, G, G)                                            # in place
@@ -463,6 +466,83 @@ def test_non_finite_activations(ng):
 
 # ---- together --------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("mx4,save8,fold", [(True, False, False), (False, True, False), (True, True, True)])
+def test_dense_layers_of_a_network(ng, mx4, save8, fold):
+    """FullLayer with 4-bit products and 8-bit saved inputs, built and run by the network driver: each layer's three
+    products against the values of its own block-scaled tensors, the rectifier derivative below, the update"""
+    from nervanagpu_amd import convnet_benchmarks as cb
+    from nervanagpu_amd.layers import DataLayer, FullLayer
+    confs = [{"layer": DataLayer, "N": 40, "C": 70, "H": 1, "W": 1}] + \
+            [{"layer": FullLayer, "nOut": n, "mx4": mx4, "save8": save8} for n in (136, 96, 33)]
+    layers = cb.build_network(ng, confs, np.float16, seed=2, fold_relu=fold)
+    layers[1].init_deltas()
+    assert [l.relu_done_above for l in layers[1:]] == [fold, fold, False]
+    y = None
+    for l in layers:
+        x = y
+        y = l.fprop(y)
+        if type(l) is FullLayer:
+            w, xin = (l._mx["W"].get(), l._mx["x"].get()) if mx4 else (l.weights.get(), x.get().reshape(l.dimI))
+            _check_product(y.get(), w.astype(np.float64), xin.astype(np.float64), "fprop", relu=True)
+            if save8:
+                assert np.array_equal(l.saved_in.get(), orc.ref_mx_round(x.get().reshape(l.dimI), "int8")[2].astype(np.float32))
+    rng = np.random.default_rng(3)
+    err = ng.array(rng.standard_normal(layers[-1].dimO).astype(np.float16))
+    for l in layers[:0:-1]:
+        e = err.get().reshape(l.dimO).astype(np.float64)
+        if not l.relu_done_above:
+            e = e * (l.fprop_out.get() > 0)
+        w0 = l.weights.get()
+        l.learning_rate = 0.0
+        err = l.bprop(err)
+        dx = err.get()
+        e16 = e.astype(np.float16).astype(np.float64)
+        if mx4:
+            wt, eq = l._mx["W^T"].get().T.astype(np.float64), l._mx["e"].get().astype(np.float64)
+            assert np.array_equal(eq, orc.ref_mx_round(e16, "fp4", 0)[2])
+        else:
+            wt, eq = w0.T.astype(np.float64), e16
+        xs = l.saved_in.get().astype(np.float64) if save8 else l.fprop_in.get().astype(np.float64)
+        if l.relu_below:
+            assert not dx[xs <= 0].any()
+            ref = wt @ eq
+            assert_fp16_within_ulp(dx, np.where(xs > 0, ref, 0.0), 0.5, "dx", np.sqrt(w0.shape[0]) * EPS32 * (np.abs(wt) @ np.abs(eq)))
+        else:
+            _check_product(dx, wt, eq, "dx")
+        _check_product(l.updat_out.get(), e16, xs.T, "dw")
+
+
+def test_shared_activation_buffers(ng):
+    """with 8-bit saved inputs two activation buffers serve a chain: the gradients are those of separate buffers"""
+    from nervanagpu_amd.layers import FullLayer
+    rng = np.random.default_rng(4)
+    N, sizes = 24, (64, 48, 80, 40)
+    x0, top = rng.standard_normal((sizes[0], N)).astype(np.float16), rng.standard_normal((sizes[-1], N)).astype(np.float16)
+    ws = [(rng.standard_normal((b, a)) * 0.2).astype(np.float16) for a, b in zip(sizes, sizes[1:])]
+    grads = []
+    for share in (False, True):
+        buffers = [ng.empty((max(sizes), N)) for _ in range(2)]
+        layers, y = [], ng.array(x0)
+        for w in ws:
+            l = FullLayer(ng, np.float16, N, w.shape[1], w.shape[0], save8=True)
+            l.init_activations(shared=buffers if share else None)
+            l.init_deltas()
+            l.init_weights()
+            l.weights.set(w)
+            if layers:
+                l.relu_below = layers[-1].relu_done_above = True
+            y = l.fprop(y)
+            layers.append(l)
+        e = ng.array(top)
+        got = []
+        for l in layers[::-1]:
+            e = l.bprop(e)
+            got += [e.get(), l.updat_out.get()]
+        grads.append(got)
+    for a, b in zip(*grads):
+        assert np.array_equal(a, b)
+
+
 def test_dense_layer_step_in_few_bits(ng):
     """forward, data gradient and weight gradient of a dense layer as a training program chains them"""
     rng = np.random.default_rng(13)
@@ -491,3 +571,143 @@ def test_dense_layer_step_in_few_bits(ng):
     # the checkpoint is close to what it stands for: half a unit of 1/64 .. 1/127 of the block's largest value (one
     # unit where that one saturates)
     assert np.abs(X8.get() - x).max() <= np.abs(x).max() / 64
+
+
+# ---- streams, graphs, far offsets -----------------------------------------------------------------
+
+def _emulated():
+    from nervanagpu_amd import _lib
+    return "emulation" in _lib.device_name()
+
+
+def _chain(ng, t):
+    """every operator once, on the tensors of `t`"""
+    ng.mx_quantize(t["x"], t["x4"])
+    ng.mx_dot(t["w4"], t["x4"], t["y"])
+    ng.fprop_act("silu", t["y"], t["a"], saved=t["q"])
+    ng.mx_dequantize(t["q"], t["z"])
+    ng.bprop_act("silu", t["q"], t["a"], t["g"])
+    ng.mx_dot(t["g"], t["q"].T, t["dw"])
+    ng.mx_dot(t["w4"], t["x"], t["y2"])
+    ng.mx_dot(t["w4"], t["few"], t["y3"])
+
+
+def _chain_tensors(ng, seed):
+    rng = np.random.default_rng(seed)
+    n, k, m = 72, 1000, 136
+    f = lambda *shape: ng.empty(shape)
+    return {"x": ng.array(rng.standard_normal((k, n)).astype(np.float16)), "x4": ng.mx_empty((k, n), axis=0, rounding=0),
+            "w4": ng.mx_array((rng.standard_normal((m, k)) * 0.1).astype(np.float16), rounding=0), "few": ng.array(rng.standard_normal((k, 3)).astype(np.float16)),
+            "y": f(m, n), "a": f(m, n), "z": f(m, n), "g": f(m, n), "q": ng.mx_empty((m, n), "int8", rounding=0),
+            "dw": ng.empty((m, m), dtype=np.float32), "y2": f(m, n), "y3": f(m, 3)}
+
+
+_CHAIN_OUT = ("y", "a", "z", "g", "dw", "y2", "y3")
+
+
+def test_on_a_stream_of_its_own(ng):
+    from nervanagpu_amd import NervanaGPU, _lib
+    t = _chain_tensors(ng, 21)
+    _chain(ng, t)
+    expect = {k: t[k].get() for k in _CHAIN_OUT}
+    stream = ctypes.c_void_p()
+    _lib.call("ng_stream_create", ctypes.byref(stream))
+    other = NervanaGPU(seed=1)
+    other.stream = stream
+    u = _chain_tensors(other, 21)
+    _lib.stream_sync(None)
+    for _ in range(3):
+        _chain(other, u)
+    for k in _CHAIN_OUT:
+        assert np.array_equal(u[k].get(), expect[k]), k
+    _lib.stream_sync(stream)
+    _lib.call("ng_stream_destroy", stream)
+
+
+def test_captured_and_replayed():
+    """the calls record nothing but kernels: a graph of all of them, replayed with new inputs between eager work"""
+    from nervanagpu_amd import NervanaGPU, _lib
+    if _emulated():
+        pytest.skip("graphs are a device matter")
+    hip = _lib.load()           # its own HIP runtime answers for the graph calls
+    vp = ctypes.c_void_p
+
+    def ok(status):
+        assert status == 0, "HIP status %d" % status
+
+    ng = NervanaGPU(seed=1)
+    stream, graph, run = vp(), vp(), vp()
+    _lib.call("ng_stream_create", ctypes.byref(stream))
+    ng.stream = stream
+    t = _chain_tensors(ng, 22)
+    _chain(ng, t)                       # the arena is there before the capture
+    _lib.stream_sync(stream)
+    ok(hip.hipStreamBeginCapture(stream, 0))
+    _chain(ng, t)
+    ok(hip.hipStreamEndCapture(stream, ctypes.byref(graph)))
+    ok(hip.hipGraphInstantiate(ctypes.byref(run), graph, None, None, ctypes.c_size_t(0)))
+    rng = np.random.default_rng(23)
+    for _ in range(3):
+        t["x"].set(rng.standard_normal(t["x"].shape).astype(np.float16))
+        _chain(ng, t)
+        expect = {k: t[k].get() for k in _CHAIN_OUT}
+        for k in _CHAIN_OUT:
+            t[k].fill(9)
+        _lib.stream_sync(stream)
+        ok(hip.hipGraphLaunch(run, stream))
+        _lib.stream_sync(stream)
+        for k in _CHAIN_OUT:
+            assert np.array_equal(t[k].get(), expect[k]), k
+    ok(hip.hipGraphExecDestroy(run))
+    ok(hip.hipGraphDestroy(graph))
+    _lib.call("ng_stream_destroy", stream)
+
+
+def test_reruns_are_bit_identical(ng):
+    rng = np.random.default_rng(24)
+    A, _ = _operand(ng, rng, (200, 4096), "fp4", 1)
+    B, _ = _operand(ng, rng, (4096, 100), "fp4", 0)
+    h = ng.array(rng.standard_normal((4096, 100)).astype(np.float16))
+    for right in (B, h, h[:, :9]):
+        C = ng.empty((200, right.shape[1]), dtype=np.float32)
+        first = ng.mx_dot(A, right, C).get()
+        for _ in range(3):
+            assert np.array_equal(ng.mx_dot(A, right, C).get(), first)
+
+
+def test_far_offsets(ng):
+    """rows 2^20 elements apart: the last ones lie beyond 2^32 elements and 2^33 bytes from the first"""
+    from nervanagpu_amd import _lib
+    if _emulated():
+        pytest.skip("needs 9 GB")
+    rows, pitch, cols = 4104, 1 << 20, 96
+    rng = np.random.default_rng(25)
+    big = ng.empty((rows, pitch))
+    w = big[:, 64:64 + cols]
+    checked = [0, 1, 2047] + list(range(4096, rows))
+    x = {r: rng.standard_normal(cols).astype(np.float16) for r in checked}
+    for r in checked:
+        _lib.memcpy_htod(w.ptr + 2 * r * pitch, x[r])
+    q = ng.mx_quantize(w, ng.mx_empty((rows, cols), "int8"))
+    got = q.get()
+    for r in checked:
+        assert np.array_equal(got[r], orc.ref_mx_round(x[r][None], "int8")[2][0].astype(np.float32))
+    tail = np.stack([x[r] for r in range(4096, rows)])
+    q0 = ng.mx_quantize(w, ng.mx_empty((rows, cols), "fp4", 0))
+    assert np.array_equal(q0.get()[4096:], orc.ref_mx_round(tail, "fp4", 0)[2].astype(np.float32))
+    # written back and read as a dense operand in place
+    ng.mx_dequantize(q, w)
+    back = np.empty(cols, dtype=np.float16)
+    for r in checked:
+        _lib.memcpy_dtoh(back, w.ptr + 2 * r * pitch)
+        assert np.array_equal(back, got[r].astype(np.float16))
+    ng.fprop_act("relu", w, w)
+    for r in checked:
+        _lib.memcpy_dtoh(back, w.ptr + 2 * r * pitch)
+        assert np.array_equal(back, np.maximum(got[r], 0).astype(np.float16))
+    E = ng.mx_array(np.eye(cols, dtype=np.float16), axis=0)
+    C = ng.empty((rows, cols))
+    ng.mx_dot(w, E, C)
+    out = C.get()
+    for r in checked:
+        assert np.array_equal(out[r], np.maximum(got[r], 0).astype(np.float16))

@@ -209,10 +209,11 @@ def test_oracle_rounds_to_the_nearest(fmt, steps):
             assert abs(v[i, j] - x[i, j]) <= best
 
 
-def _emulate(expr):
+def _emulate(expr, cus="8"):
     cmd = [sys.executable, os.path.join(ROOT, "tests", "emu", "run_on_emulator.py"), os.path.join(ROOT, "tests", "test_gpu_mx.py"),
            "-x", "-q", "-p", "no:cacheprovider", "-k", expr]
-    done = subprocess.run(cmd, cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=1500)
+    done = subprocess.run(cmd, cwd=ROOT, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, timeout=1500,
+                          env=dict(os.environ, EMU_CUS=cus))
     tail = done.stdout.decode("utf-8", "replace")[-3000:]
     assert done.returncode == 0, tail
     assert " passed" in tail and "failed" not in tail, tail
@@ -223,4 +224,9 @@ def test_conversions_on_the_emulator():
 
 
 def test_products_on_the_emulator():
-    _emulate("dense_layer or padding or nan_blocks or alpha_beta or empty or stochastic_result or outside")
+    _emulate("dense_layer or padding or nan_blocks or alpha_beta or empty or stochastic_result or outside or shared or stream_of")
+
+
+def test_large_tiles_on_the_emulator():
+    """on a chip of two CUs the 256x256 tiles cover it"""
+    _emulate("larger and 520", "2")
