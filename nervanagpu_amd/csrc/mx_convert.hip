@@ -87,7 +87,7 @@ NG_DEV void write_unit(const float (&v)[8], int line, int unit, const UnitMap& m
     const unsigned amax = mx_quad_max(abs_max_bits(v));
     const int e = mx_not_finite(amax) ? 0 : mx_exponent<FMT, SR>(amax);
     unsigned w[2];
-    mx_encode8<FMT, SR>(v, e, seed, stream, (unsigned long long)line * (unsigned)map.depth + (unsigned)unit * 8u, w);
+    mx_encode8<FMT, SR>(v, e, seed, stream, line, map.depth, unit * 8, w);
     if (mx_not_finite(amax)) w[0] = w[1] = 0;
     const size_t u = (size_t)line * map.units_per_line + unit;
     if constexpr (FMT == NG_MX_FP4) reinterpret_cast<unsigned*>(codes)[u] = w[0];
@@ -147,7 +147,7 @@ void mx_quantize_across_kernel(const T* __restrict__ A, long lda, int lines, int
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         unsigned w[2];
-        mx_encode8<FMT, SR>(v[q], e, seed, stream, (unsigned long long)(unsigned)line * (unsigned)depth + (unsigned)(i0 + q * 8), w);
+        mx_encode8<FMT, SR>(v[q], e, seed, stream, line, depth, i0 + q * 8, w);
         if (bad) w[0] = w[1] = 0;
         if constexpr (FMT == NG_MX_FP4) reinterpret_cast<unsigned*>(mine)[q] = w[0];
         else                            reinterpret_cast<mx_uint2_t*>(mine)[q] = mx_uint2_t{w[0], w[1]};
@@ -165,6 +165,38 @@ void mx_quantize_across_kernel(const T* __restrict__ A, long lda, int lines, int
     // four scale bytes at once: lines are padded to a multiple of 8, so they are there
     if (tid < 64 && line < lines)
         *reinterpret_cast<unsigned*>(scales + (long)line * scale_pitch + block0) = *reinterpret_cast<const unsigned*>(tile_scales + lane * 4);
+}
+
+// The same for matrices of few blocks, where that kernel leaves most of the chip idle: a
+// wavefront takes 16 lines, four lanes a block of 8 rows each, whose maxima meet in two
+// exchanges (4096 rows x 128 lines: 64 workgroups and 6.3 us there, 256 here)
+template <typename T, int FMT, bool SR>
+__global__ __launch_bounds__(256)
+void mx_quantize_across_small_kernel(const T* __restrict__ A, long lda, int lines, int depth, unsigned char* __restrict__ codes,
+                                     unsigned char* __restrict__ scales, long code_pitch, long scale_pitch, unsigned seed,
+                                     unsigned stream)
+{
+    constexpr int CB = FMT == NG_MX_FP4 ? 16 : 32;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int line = ((int)blockIdx.x * 4 + wave) * 16 + (lane & 15), quarter = lane >> 4;
+    const int block = (int)blockIdx.y, i0 = block * MX_BLOCK + quarter * 8;
+    float v[8];
+    const T* p = A + (long)i0 * lda + line;
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = (line < lines && i0 + i < depth) ? (float)p[(long)i * lda] : 0.0f;
+    unsigned amax = abs_max_bits(v);
+    amax = max(amax, (unsigned)__shfl_xor((int)amax, 16, 64));
+    amax = max(amax, (unsigned)__shfl_xor((int)amax, 32, 64));
+    const bool bad = mx_not_finite(amax);
+    const int e = bad ? 0 : mx_exponent<FMT, SR>(amax);
+    unsigned w[2];
+    mx_encode8<FMT, SR>(v, e, seed, stream, line, depth, i0, w);
+    if (bad) w[0] = w[1] = 0;
+    if (line >= lines) return;
+    unsigned char* out = codes + (long)line * code_pitch + (long)block * CB + quarter * (CB / 4);
+    if constexpr (FMT == NG_MX_FP4) *reinterpret_cast<unsigned*>(out) = w[0];
+    else                            *reinterpret_cast<mx_uint2_t*>(out) = mx_uint2_t{w[0], w[1]};
+    if (quarter == 0) scales[(long)line * scale_pitch + block] = (unsigned char)(bad ? 255u : mx_scale_byte<FMT>(e));
 }
 
 template <int FMT>
@@ -380,8 +412,13 @@ static int quantize(const QuantArgs& q)
         const int groups = (mx_blocks(q.depth) + 3) / 4;
         if (groups > 65535) return fail(-88, "ng_mx_quantize: depth beyond 2^23 across the rows");
         const dim3 grid((unsigned)((q.lines + 63) / 64), (unsigned)groups);
-        hipLaunchKernelGGL((mx_quantize_across_kernel<T, FMT, SR>), grid, dim3(256), 0, q.stream, (const T*)q.A, q.lda, q.lines,
-                           q.depth, (unsigned char*)q.codes, (unsigned char*)q.scales, cp, sp, q.seed, q.rng_stream);
+        if ((long)grid.x * grid.y < 2l * device_cu_count() && mx_blocks(q.depth) <= 65535)
+            hipLaunchKernelGGL((mx_quantize_across_small_kernel<T, FMT, SR>), dim3(grid.x, (unsigned)mx_blocks(q.depth)), dim3(256), 0,
+                               q.stream, (const T*)q.A, q.lda, q.lines, q.depth, (unsigned char*)q.codes, (unsigned char*)q.scales, cp, sp,
+                               q.seed, q.rng_stream);
+        else
+            hipLaunchKernelGGL((mx_quantize_across_kernel<T, FMT, SR>), grid, dim3(256), 0, q.stream, (const T*)q.A, q.lda, q.lines,
+                               q.depth, (unsigned char*)q.codes, (unsigned char*)q.scales, cp, sp, q.seed, q.rng_stream);
     }
     NG_CHECK_LAUNCH("mx quantize");
     return 0;

@@ -84,14 +84,14 @@ NG_DEV unsigned mx_int8_magnitude_stochastic(float a, unsigned r16)
 }
 
 // codes of 8 neighbouring values of one block -> 4 (fp4) or 8 (int8) bytes.
-// idx0: stream index of the first value (SR only).
-template <int FMT, bool SR>
-NG_DEV void mx_encode8(const float (&v)[8], int e, unsigned seed, unsigned stream, unsigned long long idx0, unsigned (&out)[2])
+// idx0: stream index of the first value (SR only); EVEN: it is even
+template <int FMT, bool SR, bool EVEN>
+NG_DEV void mx_encode8_words(const float (&v)[8], int e, unsigned seed, unsigned stream, unsigned long long idx0, unsigned (&out)[2])
 {
     unsigned words[5];
     bool odd = false;
     if constexpr (SR) {
-        odd = (idx0 & 1) != 0;
+        odd = !EVEN && (idx0 & 1) != 0;
         const unsigned w0 = (unsigned)(idx0 >> 1);
 #pragma unroll
         for (int i = 0; i < 4; i++) words[i] = ng_rand32(seed, stream, w0 + i);
@@ -131,6 +131,16 @@ NG_DEV void mx_encode8(const float (&v)[8], int e, unsigned seed, unsigned strea
             out[i / 4] |= ((unsigned)q & 255u) << (8 * (i & 3));
         }
     }
+}
+
+// idx0 = line * depth + i with i a multiple of 8: with an even depth it is even for
+// every line, the pairs that share a word are fixed and nothing has to be selected
+template <int FMT, bool SR>
+NG_DEV void mx_encode8(const float (&v)[8], int e, unsigned seed, unsigned stream, int line, int depth, int i, unsigned (&out)[2])
+{
+    const unsigned long long idx0 = (unsigned long long)(unsigned)line * (unsigned)depth + (unsigned)i;
+    if (!SR || (depth & 1) == 0) mx_encode8_words<FMT, SR, true>(v, e, seed, stream, idx0, out);
+    else                         mx_encode8_words<FMT, SR, false>(v, e, seed, stream, idx0, out);
 }
 
 // 8 neighbouring values (4 or 8 bytes of codes) in fp32

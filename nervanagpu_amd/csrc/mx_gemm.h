@@ -551,12 +551,16 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     const int s_read = SCALES + (wx * TX * 32 + row) * 16 + half;
 
     Block blk[TX];
-    half8_t fx_[2][TX], fd_[2][TD];
+    // few products a step cover the latency of LDS only two steps ahead: then all four steps'
+    // dense fragments have registers of their own
+    constexpr bool DEEP = TM * TN <= 4;
+    constexpr int DBUF = DEEP ? 4 : 2;
+    half8_t fx_[2][TX], fd_[DBUF][TD];
     // codes and scales of tile t (counted from the slice's first)
-    auto load_blocks = [&](int stage_off, int t, int i) {
+    auto load_blocks = [&](int stage_off, int t, int i, Block (&to)[TX]) {
         const int b = s_skip + 2 * t;                  // of the tile's first block
         const unsigned byte = *reinterpret_cast<const unsigned char*>(smem + s_read + ((b >> 4) & 1) * SLOT + i * 512 + (b & 15));
-        blk[i].load(smem + stage_off + x_off + i * 64 * Block::BYTES, x_second, b + half < blocks ? byte : 0u);
+        to[i].load(smem + stage_off + x_off + i * 64 * Block::BYTES, x_second, b + half < blocks ? byte : 0u);
     };
     // dense chunk 4 half + step of the line: the xor with the swizzle distributes
     auto load_dense = [&](int stage_off, int step, int to, int i) {
@@ -572,14 +576,14 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     };
     auto product = [&](int step, int p) {
         const int i = p / TN, j = p % TN;
-        if constexpr (X_IS_A) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fx_[step & 1][i], fd_[step & 1][j], acc[i][j], 0, 0, 0);
-        else                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fd_[step & 1][i], fx_[step & 1][j], acc[i][j], 0, 0, 0);
+        if constexpr (X_IS_A) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fx_[step & 1][i], fd_[step % DBUF][j], acc[i][j], 0, 0, 0);
+        else                  acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(fd_[step % DBUF][i], fx_[step & 1][j], acc[i][j], 0, 0, 0);
     };
     // piece c (half of a line's 8 values) of a step's expansion
-    auto expand0 = [&](int c) { if (c & 1) blk[c / 2].template expand<0, 1>(fx_[0][c / 2]); else blk[c / 2].template expand<0, 0>(fx_[0][c / 2]); };
-    auto expand1 = [&](int c) { if (c & 1) blk[c / 2].template expand<1, 1>(fx_[1][c / 2]); else blk[c / 2].template expand<1, 0>(fx_[1][c / 2]); };
-    auto expand2 = [&](int c) { if (c & 1) blk[c / 2].template expand<2, 1>(fx_[0][c / 2]); else blk[c / 2].template expand<2, 0>(fx_[0][c / 2]); };
-    auto expand3 = [&](int c) { if (c & 1) blk[c / 2].template expand<3, 1>(fx_[1][c / 2]); else blk[c / 2].template expand<3, 0>(fx_[1][c / 2]); };
+    auto expand0 = [&](int c, const Block (&from)[TX]) { if (c & 1) from[c / 2].template expand<0, 1>(fx_[0][c / 2]); else from[c / 2].template expand<0, 0>(fx_[0][c / 2]); };
+    auto expand1 = [&](int c, const Block (&from)[TX]) { if (c & 1) from[c / 2].template expand<1, 1>(fx_[1][c / 2]); else from[c / 2].template expand<1, 0>(fx_[1][c / 2]); };
+    auto expand2 = [&](int c, const Block (&from)[TX]) { if (c & 1) from[c / 2].template expand<2, 1>(fx_[0][c / 2]); else from[c / 2].template expand<2, 0>(fx_[0][c / 2]); };
+    auto expand3 = [&](int c, const Block (&from)[TX]) { if (c & 1) from[c / 2].template expand<3, 1>(fx_[1][c / 2]); else from[c / 2].template expand<3, 0>(fx_[1][c / 2]); };
 
     // Requests run NSTAGE tiles ahead, past the last tile too: those fetch zeros (every
     // chunk is out of range), so all tiles take the same path.  The waits count the codes'
@@ -596,63 +600,129 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     __syncthreads();
     int rd = 0;
 #pragma unroll
-    for (int i = 0; i < TX; i++) load_blocks(0, 0, i);
+    for (int i = 0; i < TX; i++) load_blocks(0, 0, i, blk);
 #pragma unroll
     for (int i = 0; i < TD; i++) load_dense(0, 0, 0, i);
+    if constexpr (DEEP) {
 #pragma unroll
-    for (int c = 0; c < 2 * TX; c++) expand0(c);
+        for (int i = 0; i < TD; i++) load_dense(0, 1, 1, i);
+    }
+#pragma unroll
+    for (int c = 0; c < 2 * TX; c++) expand0(c, blk);
 
     constexpr int N = TM * TN;
     constexpr int REQ = (LOADS + N - 1) / N, READ = (TD + N - 1) / N, PIECES = (2 * TX + N - 1) / N;
     constexpr int TAIL = N / 2, TAIL_PIECES = (2 * TX + (N - TAIL) - 1) / (N - TAIL);
-    for (int t = 0; t < ntiles; t++) {
-        // steps 0 .. 2, each with the dense reads and the expansion of the next between its products
+    // the group of scales after tile t's, one request at each of the group's first tiles (the
+    // slot's last group has been read: the tile before this group took its scales two barriers ago)
+    auto next_scales = [&](int t) {
+        const int b = s_skip + 2 * t, i = (b & 15) / 2 - (s_skip && b < 16 ? 1 : 0);
+        if (i < SPER) request_scales(i, (b >> 4) + 1);
+    };
+    if constexpr (DEEP) {
+        Block nblk[TX];
+        for (int t = 0; t < ntiles; t++) {
+            // steps 0 and 1 with the dense reads of 2 and 3
 #pragma unroll
-        for (int step = 0; step < 3; step++)
+            for (int step = 0; step < 2; step++)
+#pragma unroll
+                for (int p = 0; p < N; p++) {
+#pragma unroll
+                    for (int q = p * READ; q < (p + 1) * READ; q++)
+                        if (q < TD) load_dense(rd, step + 2, step + 2, q < TD ? q : 0);
+                    product(step, p);
+#pragma unroll
+                    for (int c = p * PIECES; c < (p + 1) * PIECES; c++)
+                        if (c < 2 * TX) {
+                            if (step == 0) expand1(c < 2 * TX ? c : 0, blk);
+                            else           expand2(c < 2 * TX ? c : 0, blk);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            // steps 2 and 3 with the requests into the freed stage and the reads of the next tile
+            const int freed = rd;
+            rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
+            next_scales(t);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int step = 2; step < 4; step++)
+#pragma unroll
+                for (int p = 0; p < N; p++) {
+                    product(step, p);
+                    if (step == 2) {
+#pragma unroll
+                        for (int q = p; q < TX; q += N) load_blocks(rd, t + 1, q, nblk);
+                    }
+#pragma unroll
+                    for (int q = p * READ; q < (p + 1) * READ; q++)
+                        if (q < TD) load_dense(rd, step - 2, step - 2, q < TD ? q : 0);
+                    if (step == 2) {
+#pragma unroll
+                        for (int q = p * REQ; q < (p + 1) * REQ; q++) request(q, smem + freed);
+                    }
+#pragma unroll
+                    for (int c = p * PIECES; c < (p + 1) * PIECES; c++)
+                        if (c < 2 * TX) {
+                            if (step == 2) expand3(c < 2 * TX ? c : 0, blk);
+                            else           expand0(c < 2 * TX ? c : 0, nblk);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+#pragma unroll
+            for (int i = 0; i < TX; i++) blk[i] = nblk[i];
+            advance();
+        }
+    } else {
+        for (int t = 0; t < ntiles; t++) {
+            // steps 0 .. 2, each with the dense reads and the expansion of the next between its products
+#pragma unroll
+            for (int step = 0; step < 3; step++)
+#pragma unroll
+                for (int p = 0; p < N; p++) {
+#pragma unroll
+                    for (int q = p * READ; q < (p + 1) * READ; q++)
+                        if (q < TD) load_dense(rd, step + 1, (step + 1) & 1, q < TD ? q : 0);
+                    product(step, p);
+#pragma unroll
+                    for (int c = p * PIECES; c < (p + 1) * PIECES; c++)
+                        if (c < 2 * TX) {
+                            if (step == 0) expand1(c < 2 * TX ? c : 0, blk);
+                            else if (step == 1) expand2(c < 2 * TX ? c : 0, blk);
+                            else expand3(c < 2 * TX ? c : 0, blk);
+                        }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
+            __syncthreads();
+            __builtin_amdgcn_sched_barrier(0);
+            const int freed = rd;
+            rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
+            next_scales(t);
+            __builtin_amdgcn_sched_barrier(0);
+            // last step: the next tile's codes first, the requests into the freed stage, the
+            // next tile's dense reads, and in the second half its first expansion
+#pragma unroll
+            for (int i = 0; i < TX; i++) load_blocks(rd, t + 1, i, blk);
 #pragma unroll
             for (int p = 0; p < N; p++) {
+                product(3, p);
 #pragma unroll
                 for (int q = p * READ; q < (p + 1) * READ; q++)
-                    if (q < TD) load_dense(rd, step + 1, (step + 1) & 1, q < TD ? q : 0);
-                product(step, p);
+                    if (q < TD) load_dense(rd, 0, 0, q < TD ? q : 0);
 #pragma unroll
-                for (int c = p * PIECES; c < (p + 1) * PIECES; c++)
-                    if (c < 2 * TX) {
-                        if (step == 0) expand1(c < 2 * TX ? c : 0);
-                        else if (step == 1) expand2(c < 2 * TX ? c : 0);
-                        else expand3(c < 2 * TX ? c : 0);
-                    }
+                for (int q = p * REQ; q < (p + 1) * REQ; q++) request(q, smem + freed);
+                if (p >= TAIL) {
+#pragma unroll
+                    for (int c = (p - TAIL) * TAIL_PIECES; c < (p - TAIL + 1) * TAIL_PIECES; c++)
+                        if (c < 2 * TX) expand0(c < 2 * TX ? c : 0, blk);
+                }
                 __builtin_amdgcn_sched_barrier(0);
             }
-        __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
-        __syncthreads();
-        __builtin_amdgcn_sched_barrier(0);
-        const int freed = rd, b = s_skip + 2 * t;
-        rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
-        // the group after this one, one request at each of its first tiles (the slot's last
-        // group has been read: the tile before this group took its scales two barriers ago)
-        if ((b & 15) / 2 - (s_skip && b < 16 ? 1 : 0) < SPER) request_scales((b & 15) / 2 - (s_skip && b < 16 ? 1 : 0), (b >> 4) + 1);
-        __builtin_amdgcn_sched_barrier(0);
-        // last step: the next tile's codes first, the requests into the freed stage, the
-        // next tile's dense reads, and in the second half its first expansion
-#pragma unroll
-        for (int i = 0; i < TX; i++) load_blocks(rd, t + 1, i);
-#pragma unroll
-        for (int p = 0; p < N; p++) {
-            product(3, p);
-#pragma unroll
-            for (int q = p * READ; q < (p + 1) * READ; q++)
-                if (q < TD) load_dense(rd, 0, 0, q < TD ? q : 0);
-#pragma unroll
-            for (int q = p * REQ; q < (p + 1) * REQ; q++) request(q, smem + freed);
-            if (p >= TAIL) {
-#pragma unroll
-                for (int c = (p - TAIL) * TAIL_PIECES; c < (p - TAIL + 1) * TAIL_PIECES; c++)
-                    if (c < 2 * TX) expand0(c < 2 * TX ? c : 0);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            advance();
         }
-        advance();
     }
     __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<0>::IMM);    // nothing may land in LDS behind the next barrier
 

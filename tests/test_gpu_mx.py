@@ -83,6 +83,19 @@ def test_stochastic_quantize_follows_the_stream(shape, fmt, axis):
         _check(q, x, (ng.rng_seed, ng.rng_counter))
 
 
+@pytest.mark.parametrize("fmt", ["fp4", "int8"])
+def test_many_blocks_across_the_rows(ng, fmt):
+    """large enough for the kernel that puts four blocks together (on a device), ragged at both ends"""
+    rng = np.random.default_rng(14)
+    x = rng.standard_normal((525, 8200)).astype(np.float16)
+    q = ng.mx_quantize(ng.array(x), ng.mx_empty(x.shape, fmt, 0))
+    got = q.get()
+    for cols in (slice(0, 5), slice(4000, 4006), slice(8190, 8200)):
+        _, scales, values = orc.ref_mx_round(x[:, cols], fmt, 0)
+        assert np.array_equal(got[:, cols], values.astype(np.float32))
+        assert np.array_equal(q.scales.get()[cols, :scales.shape[1]], scales)
+
+
 def test_stochastic_quantize_is_right_on_average(ng):
     """mean of n draws of a value between neighbours u apart: its variance is at most u^2 / 4n, so 6 sigma of the
     mean are 3 u / sqrt(n); the fixed point of the definition adds at most 2^-14 of a unit"""
