@@ -5,25 +5,48 @@
 
 namespace ng {
 
-// A dense operand as the kernels want it: lines of 16-byte chunks with the
-// contraction contiguous and zeros beyond it.  64 lines x 64 values through LDS.
+// A dense operand as the kernels want it: lines of 16-byte chunks with the contraction
+// contiguous and zeros beyond it.
+//
+// Lines that are contiguous but not in whole, aligned chunks: a thread a chunk.
 __global__ __launch_bounds__(256)
-void mx_pack_kernel(const unsigned short* __restrict__ X, long ld, int along, int lines, int depth, int padded,
-                    unsigned short* __restrict__ out)
+void mx_pack_along_kernel(const unsigned short* __restrict__ X, long ld, FastDiv per_line, int chunks, int depth, unsigned total,
+                          unsigned short* __restrict__ out)
+{
+    const unsigned id = blockIdx.x * 256u + threadIdx.x;
+    if (id >= total) return;
+    const int line = (int)per_line.div(id), i0 = (int)(id - (unsigned)line * (unsigned)chunks) * 8;
+    unsigned short v[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = i0 + i < depth ? X[(long)line * ld + i0 + i] : (unsigned short)0;
+    uint4_t w;
+    __builtin_memcpy(&w, v, 16);
+    *reinterpret_cast<uint4_t*>(out + (size_t)id * 8) = w;
+}
+
+// Lines across the contiguous axis: 64 lines x 64 values turned in LDS, all of a
+// thread's loads in flight at once
+__global__ __launch_bounds__(256)
+void mx_pack_across_kernel(const unsigned short* __restrict__ X, long ld, int lines, int depth, int padded,
+                           unsigned short* __restrict__ out)
 {
     __shared__ unsigned short tile[64][66];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
     const int line0 = (int)blockIdx.x * 64, i0 = (int)blockIdx.y * 64;
-#pragma unroll 4
-    for (int j = ty; j < 64; j += 4) {
-        const int line = line0 + (along ? j : tx), i = i0 + (along ? tx : j);
-        const unsigned short v = (line < lines && i < depth) ? X[along ? (long)line * ld + i : (long)i * ld + line] : (unsigned short)0;
-        tile[along ? j : tx][along ? tx : j] = v;
+    unsigned short v[16];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const int i = i0 + j * 4 + ty;
+        v[j] = (line0 + tx < lines && i < depth) ? X[(long)i * ld + line0 + tx] : (unsigned short)0;
     }
+#pragma unroll
+    for (int j = 0; j < 16; j++) tile[tx][j * 4 + ty] = v[j];
     __syncthreads();
-#pragma unroll 4
-    for (int j = ty; j < 64; j += 4)
-        if (line0 + j < lines && i0 + tx < padded) out[(long)(line0 + j) * padded + i0 + tx] = tile[j][tx];
+#pragma unroll
+    for (int j = 0; j < 16; j++) {
+        const int line = line0 + j * 4 + ty;
+        if (line < lines && i0 + tx < padded) out[(long)line * padded + i0 + tx] = tile[j * 4 + ty][tx];
+    }
 }
 
 struct MxArgs {
@@ -86,7 +109,9 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
     const int cus = device_cu_count();
     auto tiles = [&](int bm, int bn) { return (long)ceil_div(m, bm) * ceil_div(n, bn); };
     MxPlan p{128, 128, 64, 1, 0};
-    int least = 4;
+    // a slice of less than 512 values costs more in the sum of the slices than it saves
+    // (300x500 outputs of k = 600: two slices 16 us)
+    int least = 8;
     if (is_skinny(A, B, m, n)) {
         p.skinny = ((A.format == NG_MX_NONE ? m : n) + 15) / 16;
         return p;
@@ -100,6 +125,8 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
         // a contraction of few tiles is all prologue and store: more, smaller workgroups overlap
         // those (9216x4096 outputs of k = 128: 48 us on 256x256 tiles, 35 us on 128x128 with two stages)
         p.bm = p.bn = 256;
+    } else if (tiles(128, 128) <= cus / 2) {
+        p.bm = p.bn = 64;
     }
     const int out_tiles = (int)std::min<long>(tiles(p.bm, p.bn), 1 << 30);
     p.splits = choose_slices(out_tiles, ceil_div(k, p.bk), least, (size_t)m * n * 4, ws_bytes);
@@ -286,9 +313,15 @@ int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const n
                 const unsigned total = (unsigned)(bytes / 16);
                 hipLaunchKernelGGL(mx_pack_fragments_kernel, dim3((total + 255u) / 256u), dim3(256), 0, g.stream, from, o->ld, o->along,
                                    lines, k, (lines + 15) / 16, total, to);
+            } else if (o->along && (long)lines * (padded / 8) < (1L << 31)) {
+                const unsigned total = (unsigned)lines * (unsigned)(padded / 8);
+                hipLaunchKernelGGL(mx_pack_along_kernel, dim3((total + 255u) / 256u), dim3(256), 0, g.stream, from, o->ld,
+                                   FastDiv::make((unsigned)padded / 8u), padded / 8, k, total, to);
+            } else if (!o->along) {
+                hipLaunchKernelGGL(mx_pack_across_kernel, dim3((unsigned)ceil_div(lines, 64), (unsigned)ceil_div(padded, 64)), dim3(256), 0,
+                                   g.stream, from, o->ld, lines, k, padded, to);
             } else {
-                hipLaunchKernelGGL(mx_pack_kernel, dim3((unsigned)ceil_div(lines, 64), (unsigned)ceil_div(padded, 64)), dim3(256), 0,
-                                   g.stream, from, o->ld, o->along, lines, k, padded, to);
+                return fail(-98, "ng_mx_gemm: dense operand of 2^34 or more values that is not laid out in whole chunks");
             }
             NG_CHECK_LAUNCH("mx pack");
             o->codes = end;

@@ -113,8 +113,9 @@ struct MxAcrossTile {
     static constexpr int PITCH = LINES * 2;
     static constexpr int CHUNKS = 64 * CPR;
     static constexpr int BYTES = 64 * PITCH;
-    static_assert(CPR % 16 == 0, "the swizzle permutes four groups of 64 bytes");
-    static __device__ __forceinline__ int swizzle(int i) { return (i & 3) * 4; }
+    static_assert(CPR == 8 || CPR % 16 == 0, "rows of 128 bytes or whole periods of 256");
+    // rows of 128 bytes take turns in a period by themselves
+    static __device__ __forceinline__ int swizzle(int i) { return CPR == 8 ? ((i >> 1) & 1) * 4 : (i & 3) * 4; }
 };
 
 template <class Tile, int NT>
@@ -469,9 +470,9 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     constexpr int TM = X_IS_A ? TX : TD, TN = X_IS_A ? TD : TX, WTN = TN * 32;
     using Block = MxBlock<FMT>;
     using TileX = MxTile<BX, 2 * Block::BYTES>;
-    using TileD = std::conditional_t<ACROSS, MxAcrossTile<ACROSS ? BD : 128>, MxTile<BD, 128>>;
+    using TileD = std::conditional_t<ACROSS, MxAcrossTile<BD>, MxTile<BD, 128>>;
     using FX = MxFetch<TileX, NT>;
-    using FD = std::conditional_t<ACROSS, MxAcrossFetch<MxAcrossTile<ACROSS ? BD : 128>, NT>, MxFetch<MxTile<BD, 128>, NT>>;
+    using FD = std::conditional_t<ACROSS, MxAcrossFetch<MxAcrossTile<BD>, NT>, MxFetch<MxTile<BD, 128>, NT>>;
     // scales: groups of 16 blocks (8 tiles), four lanes a line, in a ring of two slots
     constexpr int SPER = BX / 16 / WAVES, SLOT = BX * 16;
     static_assert(BX % (16 * WAVES) == 0 && SPER <= 4, "scale requests must divide evenly over wavefronts");
@@ -732,7 +733,7 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     EpilogueBands<TM, TN, WTN, EPITCH, 0>::run(acc, stage, lane, m0 + wm * TM * 32, n0 + wn * WTN, 0, split, epi);
 }
 
-// tile: 256 or 128 lines of either side; defined in mx_mix.hip for the epilogues of products
+// tile: 256, 128 or 64 lines of either side; defined in mx_mix.hip for the epilogues of products
 template <int FMT, class Epi>
 void launch_mix(bool x_is_a, bool across, int tile, const MxSide& x, const MxSide& d, const Epi& epi, const CoreShape& s, dim3 grid,
                 hipStream_t stream);

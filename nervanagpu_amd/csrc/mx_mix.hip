@@ -9,6 +9,7 @@ template <int FMT, bool X_IS_A, bool ACROSS, class Epi>
 static void launch(int tile, const MxSide& x, const MxSide& d, const Epi& epi, const CoreShape& s, dim3 grid, hipStream_t stream)
 {
     if (tile == 256)         hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, ACROSS, 256, 256, 4, 2, 3, Epi>), grid, dim3(512), 0, stream, x, d, epi, s);
+    else if (tile == 64)     hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, ACROSS, 64, 64, 2, 1, 4, Epi>), grid, dim3(128), 0, stream, x, d, epi, s);
     else if (s.k_tiles <= 2) hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, ACROSS, 128, 128, 2, 2, 2, Epi>), grid, dim3(256), 0, stream, x, d, epi, s);
     else                     hipLaunchKernelGGL((mxmix_kernel<FMT, X_IS_A, ACROSS, 128, 128, 2, 2, 3, Epi>), grid, dim3(256), 0, stream, x, d, epi, s);
 }
