@@ -264,6 +264,7 @@ static int check_product(int c_dtype, int m, int n, int k, const ng_mx_operand* 
     if (!ok) return fail(-97, "ng_mx_gemm: formats %d and %d do not multiply (fp4 by fp4, or one dense fp16 operand)", A->format, B->format);
     if (k >= (1 << 21)) return fail(-98, "ng_mx_gemm: contraction of 2^21 or more");
     if ((long)m * n >= (1L << 32)) return fail(-99, "ng_mx_gemm: output of 2^32 or more elements");
+    if (m >= (1 << 26) || n >= (1 << 26)) return fail(-99, "ng_mx_gemm: output of 2^26 or more rows or columns");
     return 0;
 }
 
@@ -298,6 +299,9 @@ int ng_mx_gemm(int c_dtype, int m, int n, int k, const ng_mx_operand* A, const n
                     workspace ? workspace_bytes : (size_t)0);
     MxArgs g{c_dtype, m, n, k, *A, *B, C, ldc, alpha, beta, flags, seed, rng_stream,
              (char*)workspace, workspace_bytes, (hipStream_t)stream};
+    // the pitch of a single line has no meaning and may be anything
+    if (m == 1 && g.A.along) g.A.ld = k;
+    if (n == 1 && g.B.along) g.B.ld = k;
     // dense operands that are not laid out for the kernels are copied behind the slices
     char* end = g.ws + need;
     int lines = m;

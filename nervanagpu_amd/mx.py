@@ -62,9 +62,10 @@ class MXTensor(object):
             assert given is not None and given.dtype.type is np.uint8 and given.shape == d and given.is_contiguous, \
                 "%s of this MXTensor are a contiguous uint8 tensor of %s" % (what, d)
             assert not self.size or given.ptr % 16 == 0, "%s must be 16-byte aligned" % what
-        self.codes, self.scales = codes, scales
+        # fixed for the tensor's life, like a GPUTensor's memory
+        self._codes, self._scales = codes, scales
         self.nbytes = codes.nbytes + scales.nbytes
-        self._operand = None
+        self._operand = _lib.MxOperand(self.fmt_code, 1, 0, codes.ptr if self.size else None, scales.ptr if self.size else None)
 
     def __str__(self):
         return "MXTensor(%s) name:%s shape:%s axis:%d rounding:%s" % (self.fmt, self.name, self.shape, self.axis, self.rounding)
@@ -99,9 +100,14 @@ class MXTensor(object):
             self.backend.mx_dequantize(self, out)
         return out.get()
 
+    @property
+    def codes(self):
+        return self._codes
+
+    @property
+    def scales(self):
+        return self._scales
+
     def operand(self):
         """this tensor as an operand of ng_mx_gemm"""
-        if self._operand is None:
-            self._operand = _lib.MxOperand(self.fmt_code, 1, 0, self.codes.ptr if self.size else None,
-                                           self.scales.ptr if self.size else None)
         return self._operand

@@ -716,7 +716,7 @@ class NervanaGPU(object):
         assert not A.size, "one dimension of %s must be contiguous" % what
         return depth, 1
 
-    def mx_quantize(self, A, out, repeat=1):
+    def mx_quantize(self, A, out):
         """out = A in blocks of 32 values that share a power of two.  A: fp16 or fp32
         matrix with one contiguous dimension.  Rounds to the nearest code (ties to
         even), or stochastically if out.rounding is set: then every value is right on
@@ -725,9 +725,7 @@ class NervanaGPU(object):
         if A.dtype.type not in _FLOATS:
             raise TypeError("Only floating point tensors can be quantized.")
         ld, along = self._mx_dense(A, out.axis, "A")
-        if not out.size:
-            return out
-        for r in range(repeat):
+        if out.size:
             flags, (seed, sid) = (_lib.FLAG_SR, self._next_rng_stream()) if out.rounding else (0, (0, 0))
             _lib.call("ng_mx_quantize", out.fmt_code, _DTYPE_CODE[A.dtype], A.ptr, ld, along, out.lines, out.depth,
                       out.codes.ptr, out.scales.ptr, flags, seed, sid, self.stream)
@@ -831,15 +829,16 @@ class NervanaGPU(object):
         codes = scales = None
         if saved is not None:
             assert type(saved) is MXTensor and saved.shape == first.shape, "the checkpoint must match the operands"
-            if saved.fmt != "int8" or saved.axis != 1 or saved.rounding:
-                raise ValueError("a checkpoint of activations is an int8 MXTensor with axis 1 and nearest rounding")
+            if saved.fmt != "int8" or saved.axis != 1:
+                raise ValueError("a checkpoint of activations is an int8 MXTensor with axis 1")
             if saved.size:
                 codes, scales = saved.codes.ptr, saved.scales.ptr
         return code, _DTYPE_CODE[first.dtype], first.shape[0], first.shape[1], codes, scales, lds
 
     def fprop_act(self, op, I, O, saved=None):
         """
-        O = op(I), and saved (an MXTensor, fmt "int8", axis 1) = I, in one pass.
+        O = op(I), and saved (an MXTensor, fmt "int8", axis 1) = I rounded to the
+        nearest, in one pass.
 
         op: "relu", "sig", "tanh", "silu" (x sig(x)) or "gelu" (x times the normal
         distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous; O may be I

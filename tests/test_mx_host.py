@@ -40,6 +40,8 @@ def test_layout():
     ng = NervanaGPU()
     q = fake_mx(ng, (5, 70), axis=0)
     assert (q.lines, q.depth) == (70, 5) and q.codes.shape == (70, 16) and q.scales.shape == (70, 8)
+    with pytest.raises(AttributeError):
+        q.codes = q.scales          # the memory is fixed
     t = q.T
     assert t.shape == (70, 5) and t.axis == 1 and t.codes is q.codes and len(t) == 70 and t.nbytes == q.nbytes
 
@@ -123,7 +125,7 @@ def test_activation_refusals(calls):
         ng.fprop_act("softplus", z, z)
     with pytest.raises(ValueError):
         ng.bprop_act("softplus", q, z, z)
-    for bad in (fake_mx(ng, (8, 64)), fake_mx(ng, (8, 64), "int8", 0), fake_mx(ng, (8, 64), "int8", rounding=1)):
+    for bad in (fake_mx(ng, (8, 64)), fake_mx(ng, (8, 64), "int8", 0)):
         with pytest.raises(ValueError):
             ng.fprop_act("relu", z, z, saved=bad)
         with pytest.raises(ValueError):
@@ -183,6 +185,7 @@ def test_c_abi_refusals():
     assert gemm(operand(1, codes=0x100004), half) < 0
     assert gemm(four, operand(0, 1, 60)) < 0 and gemm(four, operand(0, 0, 3)) < 0
     assert gemm(four, half, k=1 << 21) < 0
+    assert gemm(four, half, m=1 << 26) < 0
     assert gemm(four, four, m=1 << 17, n=1 << 16, ldc=1 << 16) < 0
     # a dense operand that has to be copied first needs room
     odd = operand(0, 1, 65, 0x100002)
