@@ -1,6 +1,11 @@
 // Conversions between dense and block-scaled matrices, and the activation
-// functions that keep an 8-bit checkpoint of their input.  All of them are bound by
-// memory: each value is read once and written once.
+// functions that keep an 8-bit checkpoint of their input.  All of them read each value once
+// and write it once.  fp16 of 16384x8192, against 4.9 TB/s of a large copy:
+//   backward gelu from the checkpoint   115 us, 675 MB, 5.9 TB/s: memory
+//   fp4 to fp16                          61 us, 340 MB, 5.5 TB/s: memory
+//   fp16 to fp4, stochastic             118 us, 340 MB, 2.9 TB/s: the vector unit (two 32-bit
+//                                        products of the random word a pair of values, 10 operations a value)
+// and at 4096x128 the launch: 2.3 to 3.9 us a kernel.
 #include "mx_format.h"
 
 #include <algorithm>

@@ -119,13 +119,16 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
     if (is_44(A, B)) {
         p.bk = 256;
         least = 2;
-        if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2) p.bm = p.bn = 256;
+        // 256 x 256 where they cover half the chip and more than two of their tiles follow each other; 64 x 64 where
+        // 128 x 128 would leave half of it idle (1111x777 outputs of k = 2500: 20 us and a sum of slices, 12 us without)
+        if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2 && k > 512) p.bm = p.bn = 256;
         else if (tiles(128, 128) <= cus / 2) p.bm = p.bn = 64;
     } else if (m >= 256 && n >= 256 && tiles(256, 256) > cus / 2 && k > 256) {
         // a contraction of few tiles is all prologue and store: more, smaller workgroups overlap
         // those (9216x4096 outputs of k = 128: 48 us on 256x256 tiles, 35 us on 128x128 with two stages)
         p.bm = p.bn = 256;
     } else if (tiles(128, 128) <= cus / 2) {
+        // a few workgroups wait out each tile's latency: four times as many (512^3 11.0 -> 7.5 us)
         p.bm = p.bn = 64;
     }
     const int out_tiles = (int)std::min<long>(tiles(p.bm, p.bn), 1 << 30);
@@ -209,9 +212,9 @@ static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
     s.tiles_n = ceil_div(g.n, p.bn);
     const int tiles = s.tiles_m * s.tiles_n;
     const dim3 grid(grid_tiles(tiles, s.splits), grid_slices(tiles, s.splits), 1);
-    ScaleStoreEpilogue<T> epi{(T*)g.C, 0, g.ldc, g.m, g.n, g.alpha, g.beta, (g.flags & NG_FLAG_RELU) ? 1u : 0u,
-                              mx_sr_bits(g.flags, g.c_dtype), g.seed, g.rng_stream,
-                              (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u};
+    const MxStoreEpilogue<T> epi{{(T*)g.C, 0, g.ldc, g.m, g.n, g.alpha, g.beta, (g.flags & NG_FLAG_RELU) ? 1u : 0u,
+                                  mx_sr_bits(g.flags, g.c_dtype), g.seed, g.rng_stream,
+                                  (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u}};
     if constexpr ((FA == NG_MX_FP4) != (FB == NG_MX_FP4)) {
         if (p.skinny) return launch_skinny<FA == NG_MX_FP4>(g, p.skinny, FA == NG_MX_FP4 ? a : b, FA == NG_MX_FP4 ? b : a, epi);
     }
@@ -219,10 +222,10 @@ static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
         launch_tiles<T, FA, FB>(g, p, a, b, epi, s, grid);
         NG_CHECK_LAUNCH("mx product");
     } else {
-        PartialEpilogue pe{(float*)g.ws, g.m, g.n, 1, (g.n % 8 == 0) ? 1u : 0u};
+        const MxPartialEpilogue pe{{(float*)g.ws, g.m, g.n, 1, (g.n % 8 == 0) ? 1u : 0u}};
         launch_tiles<T, FA, FB>(g, p, a, b, pe, s, grid);
         NG_CHECK_LAUNCH("mx product slices");
-        launch_splitk_reduce<T, ScaleStoreEpilogue<T>>((const float*)g.ws, s.splits, 1, g.m, g.n, epi, g.stream);
+        launch_splitk_reduce<T, MxStoreEpilogue<T>>((const float*)g.ws, s.splits, 1, g.m, g.n, epi, g.stream);
         NG_CHECK_LAUNCH("mx product sum");
     }
     return 0;

@@ -7,6 +7,14 @@
 //   mxmix_kernel  fp4 or int8 . fp16 on v_mfma 32x32x16 f16: codes travel through LDS as
 //                 they are and become fp16 in registers, in the shadow of the matrix pipe.
 //
+// What bounds them.  fp4 . fp4 at 8192^3: 280..300 us, 3700..3900 TFLOP/s, where a loop of
+// nothing but the instruction on random operands reaches 6400 (power; 8850 on zeros) and
+// the library's product 3175.  What it took: 256 x 256 tiles of 256 values (128-byte lines: half the
+// memory requests of 128 values, 310 -> 298 us), scales fetched for four lanes' dwords of a line
+// at once (340 -> 310 us: a dword a line made as many requests as the codes), and every tile on one
+// path without a drain loop (454 -> 345 us).  fp16 . int8 at 4096x8192x8000: 460 us, 1140
+// TFLOP/s (a plain fp16 product of the library: 415 us); fp16 . fp4 there 430 us.
+//
 // Both operands lie with the contraction contiguous (a line per row of A / column of
 // B).  Tiles are staged with loads that write LDS directly; a tile's scales (4 blocks,
 // a dword, per line) are staged beside its codes.  The order of fetching is that of
@@ -732,6 +740,40 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     const int wm = X_IS_A ? wx : wd, wn = X_IS_A ? wd : wx;
     EpilogueBands<TM, TN, WTN, EPITCH, 0>::run(acc, stage, lane, m0 + wm * TM * 32, n0 + wn * WTN, 0, split, epi);
 }
+
+// The stores of a product: those of ScaleStoreEpilogue and PartialEpilogue, except that 8
+// neighbouring values of a row that is not 16-byte aligned (an odd row length) still go out
+// in wide stores, which the hardware takes at any alignment, instead of one by one
+// (4001x5003 fp32 outputs of fp16 by int8, k = 64: 64 us one by one, 28 us so).
+template <typename T>
+struct MxStoreEpilogue : ScaleStoreEpilogue<T> {
+    typedef ScaleStoreEpilogue<T> Base;
+    typedef typename Base::bits_t bits_t;
+    __device__ __forceinline__ void store8(int i, int j0, int z, int split, const float (&acc)[8]) const
+    {
+        if (this->vec || i >= this->m || j0 + 8 > this->n) {
+            Base::store8(i, j0, z, split, acc);
+            return;
+        }
+        bits_t* p = reinterpret_cast<bits_t*>(this->C + (long)i * this->ldc + j0);
+        bits_t out[8];
+        if (this->beta != 0.0f) __builtin_memcpy(out, p, sizeof(out));
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            float v = this->scale(acc[e]);
+            if (this->beta != 0.0f) v += this->beta * StoreBits<T>::widen(out[e]);
+            out[e] = StoreBits<T>::round(v, this->sr_bits, this->seed, this->stream, this->rng_index(i, j0 + e, z));
+        }
+        __builtin_memcpy(p, out, sizeof(out));
+    }
+};
+struct MxPartialEpilogue : PartialEpilogue {
+    __device__ __forceinline__ void store8(int i, int j0, int z, int split, const float (&acc)[8]) const
+    {
+        if (vec || i >= m || j0 + 8 > n) PartialEpilogue::store8(i, j0, z, split, acc);
+        else                             __builtin_memcpy(ws + ((long)split * m + i) * (long)n + j0, acc, sizeof(acc));
+    }
+};
 
 // tile: 256, 128 or 64 lines of either side; defined in mx_mix.hip for the epilogues of products
 template <int FMT, class Epi>

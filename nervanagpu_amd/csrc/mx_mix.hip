@@ -30,9 +30,9 @@ void launch_mix(bool x_is_a, bool across, int tile, const MxSide& x, const MxSid
 #ifndef NG_MX_MIX_FORMAT
 #define NG_MX_MIX_FORMAT NG_MX_FP4
 #endif
-NG_MIX(NG_MX_MIX_FORMAT, ScaleStoreEpilogue<_Float16>);
-NG_MIX(NG_MX_MIX_FORMAT, ScaleStoreEpilogue<float>);
-NG_MIX(NG_MX_MIX_FORMAT, PartialEpilogue);
+NG_MIX(NG_MX_MIX_FORMAT, MxStoreEpilogue<_Float16>);
+NG_MIX(NG_MX_MIX_FORMAT, MxStoreEpilogue<float>);
+NG_MIX(NG_MX_MIX_FORMAT, MxPartialEpilogue);
 #undef NG_MIX
 
 }  // namespace ng

@@ -1,4 +1,7 @@
-// fp4 by a few fp16 lines (one token, some streams): bound by reading the codes once.
+// fp4 by a few fp16 lines (one token, some streams): bound by reading the codes once, and for
+// small matrices by the launch (4096x4096 by one line: 5.1 us, of which the 9 MB of codes are
+// 1.8 at the rate of a copy; 4096x25088 by 16 lines: 19 us, codes 11, the rest mostly the 16 dense
+// lines that each workgroup reads from L2).  On 128x128 tiles these took 17 and 43 us.
 //
 // A workgroup owns 16 lines of codes and the whole contraction, which its WAVES
 // wavefronts cut into equal shares; their sums meet in LDS, so there is one launch and no
