@@ -127,8 +127,10 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
         // a contraction of few tiles is all prologue and store: more, smaller workgroups overlap
         // those (9216x4096 outputs of k = 128: 48 us on 256x256 tiles, 35 us on 128x128 with two stages)
         p.bm = p.bn = 256;
-    } else if (tiles(128, 128) <= cus / 2) {
-        // a few workgroups wait out each tile's latency: four times as many (512^3 11.0 -> 7.5 us)
+    } else if (tiles(128, 128) <= cus / 2 && tiles(128, 128) * std::max(1, ceil_div(k, 64) / least) < cus) {
+        // a few workgroups wait out each tile's latency: four times as many where slices of the contraction do not
+        // make up for them (512^3 7.5 us, 11.0 on 128x128 tiles; 600x900 outputs of k = 8000 66 us, 32 on 128x128 in slices;
+        // 4096x48 of k = 4096 14.7 and 15.5)
         p.bm = p.bn = 64;
     }
     const int out_tiles = (int)std::min<long>(tiles(p.bm, p.bn), 1 << 30);
