@@ -78,8 +78,11 @@ struct MxTile {
 // lie behind the descriptor's end, chunks behind a line's last take an offset that does.
 template <class Tile, int NT>
 struct MxFetch {
-    static constexpr int DATA = Tile::CHUNKS / NT, STEP = NT / Tile::CPR;
-    static_assert(Tile::CHUNKS % NT == 0 && NT % Tile::CPR == 0, "tile chunks must divide evenly over threads");
+    // PART: the tile has fewer chunks than the workgroup threads; its first WAVES_WITH wavefronts bring it
+    static constexpr bool PART = Tile::CHUNKS < NT;
+    static constexpr int WAVES_WITH = PART ? Tile::CHUNKS / 64 : NT / 64;
+    static constexpr int DATA = PART ? 1 : Tile::CHUNKS / NT, STEP = NT / Tile::CPR;
+    static_assert((PART ? Tile::CHUNKS % 64 : Tile::CHUNKS % NT) == 0 && NT % Tile::CPR == 0, "tile chunks must divide evenly over threads");
     static_assert(DATA == 1 || (STEP / Tile::LP) % Tile::CPR == 0, "requests must be whole periods of the swizzle");
     const char* base;        // of the next tile
     int bytes;               // from there to the end of the operand, 2^31 - 1 if that is further
@@ -485,7 +488,7 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     constexpr int SPER = BX / 16 / WAVES, SLOT = BX * 16;
     static_assert(BX % (16 * WAVES) == 0 && SPER <= 4, "scale requests must divide evenly over wavefronts");
     constexpr int STAGE = TileX::BYTES + TileD::BYTES, SCALES = NSTAGE * STAGE;
-    constexpr int LOADS = FX::DATA + FD::DATA;
+    constexpr int LOADS = FX::DATA + FD::DATA;          // one less for wavefronts without codes to bring (PART)
     constexpr int EPITCH = WTN * 4 + 16, EPI_BYTES = 32 * EPITCH;
     constexpr int SMEM = SCALES + 2 * SLOT > EPI_BYTES * WAVES ? SCALES + 2 * SLOT : EPI_BYTES * WAVES;
     static_assert(SMEM <= 160 * 1024, "tile stages exceed the LDS of a compute unit");
@@ -510,8 +513,20 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     fx.init(x, x0, t_begin, tid);
     fd.init(d, d0, t_begin, tid);
     auto request = [&](int q, char* st) {
-        if (q < FX::DATA) fx.issue(q, fx.lane_offset(), st, wave);
+        if (q < FX::DATA) { if constexpr (!FX::PART) fx.issue(q, fx.lane_offset(), st, wave); }
         else if (q < LOADS) fd.issue(q - FX::DATA, fd.lane_offset(), st + TileX::BYTES, wave);
+    };
+    // codes that part of the wavefronts bring are requested before the tile's dense chunks
+    auto request_part = [&](char* st) {
+        if constexpr (FX::PART) {
+            if (wave < FX::WAVES_WITH) fx.issue(0, fx.lane_offset(), st, wave);
+        }
+    };
+    // at most `tiles` tiles' requests outstanding
+    auto wait_tiles = [&](auto tiles) {
+        constexpr int T = decltype(tiles)::value;
+        if (!FX::PART || wave < FX::WAVES_WITH) __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<T * LOADS>::IMM);
+        else                                    __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<T * (LOADS - 1)>::IMM);
     };
     auto advance = [&]() {
         fx.advance();
@@ -601,11 +616,12 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     for (int i = 0; i < SPER; i++) request_scales(i, 0);
 #pragma unroll
     for (int p = 0; p < NSTAGE; p++) {
+        request_part(smem + p * STAGE);
 #pragma unroll
         for (int q = 0; q < LOADS; q++) request(q, smem + p * STAGE);
         advance();
     }
-    __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 1) * LOADS>::IMM);
+    wait_tiles(std::integral_constant<int, NSTAGE - 1>{});
     __syncthreads();
     int rd = 0;
 #pragma unroll
@@ -648,13 +664,14 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
+            wait_tiles(std::integral_constant<int, NSTAGE - 2>{});
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
             // steps 2 and 3 with the requests into the freed stage and the reads of the next tile
             const int freed = rd;
             rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
             next_scales(t);
+            request_part(smem + freed);
             __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int step = 2; step < 4; step++)
@@ -704,12 +721,13 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
                         }
                     __builtin_amdgcn_sched_barrier(0);
                 }
-            __builtin_amdgcn_s_waitcnt(WaitVmLgkm0<(NSTAGE - 2) * LOADS>::IMM);
+            wait_tiles(std::integral_constant<int, NSTAGE - 2>{});
             __syncthreads();
             __builtin_amdgcn_sched_barrier(0);
             const int freed = rd;
             rd = (rd + STAGE == NSTAGE * STAGE) ? 0 : rd + STAGE;
             next_scales(t);
+            request_part(smem + freed);
             __builtin_amdgcn_sched_barrier(0);
             // last step: the next tile's codes first, the requests into the freed stage, the
             // next tile's dense reads, and in the second half its first expansion
