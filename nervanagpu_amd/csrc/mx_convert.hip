@@ -9,6 +9,7 @@
 #include "mx_format.h"
 
 #include <algorithm>
+#include <climits>
 
 namespace ng {
 
@@ -376,6 +377,8 @@ static int check_matrix(const char* what, int dtype, const void* p, long ld, int
 {
     if (dtype != NG_F16 && dtype != NG_F32) return fail(-80, "%s: the dense matrix must be fp16 or fp32", what);
     if (lines < 0 || depth < 0) return fail(-81, "%s: negative extent", what);
+    // grids and blocks are counted in int, rounded up
+    if (lines > INT_MAX - 256 || depth > INT_MAX - 256) return fail(-87, "%s: extent of 2^31 - 256 or more", what);
     if (!lines || !depth) return 1;
     if (!p) return fail(-82, "%s: null matrix", what);
     if (ld < (along ? depth : lines) && (along ? lines : depth) > 1) return fail(-83, "%s: rows overlap (pitch %ld)", what, ld);

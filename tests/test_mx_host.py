@@ -196,6 +196,21 @@ def test_c_abi_refusals():
         assert gemm(four, odd, k=65, ws=vp(0x100008), nbytes=need) < 0
 
 
+@pytest.mark.parametrize("along", [0, 1])
+@pytest.mark.parametrize("extents", [(2 ** 31 - 1, 1), (1, 2 ** 31 - 1), (2 ** 31 - 256, 1)])
+def test_extents_that_round_up_past_an_int_are_refused(along, extents):
+    """rounding such an extent up to whole blocks or workgroups leaves the range of int"""
+    lib = _lib.load()
+    P = ctypes.c_void_p(0x100000)
+    lines, depth = extents
+    ld, want = max(extents), -87
+    assert lib.ng_mx_quantize(1, 0, P, ld, along, lines, depth, P, P, 0, 0, 0, None) == want
+    assert lib.ng_mx_dequantize(1, P, P, lines, depth, 0, P, ld, along, None) == want
+    if along:
+        assert lib.ng_act_fprop(0, 0, lines, depth, P, ld, P, ld, None, None, None) == want
+        assert lib.ng_act_bprop(0, 0, lines, depth, P, P, P, ld, P, ld, None) == want
+
+
 @pytest.mark.parametrize("fmt,steps", [("fp4", None), ("int8", 1.0)])
 def test_oracle_rounds_to_the_nearest(fmt, steps):
     """the oracle itself: no value of the format is nearer, and packing loses nothing"""
