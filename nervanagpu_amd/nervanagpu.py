@@ -772,6 +772,7 @@ class NervanaGPU(object):
         (m, k), n = A.shape, B.shape[1]
         assert C.shape == (m, n) and B.shape[0] == k
         ldc, by_rows = self._mx_dense(C, 1, "C")
+        assert ldc < 2 ** 31, "rows of C are too far apart"
         if not by_rows:
             # columns contiguous: the transposed product
             m, n, a, b = n, m, b, a

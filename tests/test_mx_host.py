@@ -118,6 +118,16 @@ def test_dot_refusals(calls):
     assert not calls
 
 
+def test_result_with_rows_too_far_apart_is_refused(calls):
+    """the pitch of C travels as an int: 2^32 + 16 would arrive as 16"""
+    ng = NervanaGPU()
+    A, B = fake_mx(ng, (8, 64)), fake_mx(ng, (64, 16), axis=0)
+    for wide in (fake(ng, (8, 2 ** 32 + 16))[:, :16], fake(ng, (16, 2 ** 31))[:, :8].T):
+        with pytest.raises(AssertionError, match="apart"):
+            ng.mx_dot(A, B, wide)
+    assert not calls
+
+
 def test_activation_refusals(calls):
     ng = NervanaGPU()
     z, q = fake(ng, (8, 64)), fake_mx(ng, (8, 64), "int8")
