@@ -263,7 +263,8 @@ int ng_mx_dequantize(int format, const void* codes, const void* scales, int line
  *   ng_act_fprop  O = f(I); codes and scales, unless NULL, receive I; O may be I
  *   ng_act_bprop  gradI = E * f'(the values of the checkpoint); gradI may be E
  * E, O and gradI have the dtype (NG_F16 or NG_F32) of I; ldi, ldo, lde, ldg are row
- * pitches in elements. */
+ * pitches in elements.  NaN stays NaN, under relu too: a block of the checkpoint that holds
+ * one infinity or NaN makes its 32 values of gradI NaN. */
 enum ng_act { NG_ACT_RELU = 0, NG_ACT_SIG = 1, NG_ACT_TANH = 2, NG_ACT_SILU = 3, NG_ACT_GELU = 4 };
 int ng_act_fprop(int act, int dtype, int rows, int cols, const void* I, long ldi, void* O, long ldo,
                  void* codes, void* scales, void* stream);

@@ -300,7 +300,7 @@ template <int ACT, bool FAST>
 NG_DEV float act_value(float z)
 {
     float density;
-    if constexpr (ACT == NG_ACT_RELU) return fmaxf(z, 0.0f);
+    if constexpr (ACT == NG_ACT_RELU) return z <= 0.0f ? 0.0f : z;     // NaN stays NaN
     if constexpr (ACT == NG_ACT_SIG)  return act_logistic<FAST>(z);
     if constexpr (ACT == NG_ACT_TANH) return tanhf(z);
     if constexpr (ACT == NG_ACT_SILU) return z * act_logistic<FAST>(z);
@@ -310,7 +310,8 @@ NG_DEV float act_value(float z)
 template <int ACT, bool FAST>
 NG_DEV float act_slope(float z)
 {
-    if constexpr (ACT == NG_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+    // a block that is marked NaN has no derivative, under relu as under the others
+    if constexpr (ACT == NG_ACT_RELU) return z > 0.0f ? 1.0f : z <= 0.0f ? 0.0f : z;
     if constexpr (ACT == NG_ACT_SIG) { const float s = act_logistic<FAST>(z); return s * (1.0f - s); }
     if constexpr (ACT == NG_ACT_TANH) { const float t = tanhf(z); return 1.0f - t * t; }
     if constexpr (ACT == NG_ACT_SILU) { const float s = act_logistic<FAST>(z); return s * (1.0f + z * (1.0f - s)); }

@@ -261,8 +261,9 @@ class FullLayer(Layer):
             their gradient stay as they are.
     save8   the input is kept for the backward pass in 8 bits (saved_in): the weight
             gradient, and with relu_below the rectifier derivative of the layer
-            below, are computed from what those stand for.  The fp16 input may be
-            overwritten once fprop has returned, so layers may share activation
+            below, are computed from what those stand for: NaN for the 32 values of a
+            block that holds an infinity or a NaN.  The fp16 input may be overwritten
+            once fprop has returned, so layers may share activation
             buffers (init_activations(shared=...)).
     """
 

@@ -851,7 +851,8 @@ class NervanaGPU(object):
 
     def bprop_act(self, op, saved, E, grad_I):
         """grad_I = E * op'(saved): the derivative is taken at the values the 8-bit
-        checkpoint of fprop_act stands for.  grad_I may be E."""
+        checkpoint of fprop_act stands for, NaN where its block holds an infinity or
+        a NaN (under relu too).  grad_I may be E."""
         assert saved is not None, "bprop_act needs the checkpoint of fprop_act"
         code, dtype, rows, cols, codes, scales, (lde, ldg) = self._act_operands(op, (E, grad_I), saved)
         if E.size:

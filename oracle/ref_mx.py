@@ -120,7 +120,7 @@ def ref_act(op, z):
 def ref_act_slope(op, z):
     z = np.asarray(z, dtype=np.float64)
     if op == "relu":
-        return (z > 0).astype(np.float64)
+        return np.where(np.isnan(z), np.nan, z > 0)
     if op == "tanh":
         return 1.0 - np.tanh(z) ** 2
     if op == "gelu":
