@@ -280,7 +280,8 @@ int ng_act_bprop(int act, int dtype, int rows, int cols, const void* codes, cons
  * nothing if they came from fp16.
  * Dense operand: format NG_MX_NONE, codes = the matrix, element (line, i) at
  * [line * ld + i] (along = 1) or [i * ld + line] (along = 0).
- * flags, seed, rng_stream and the order of operations are those of ng_gemm.
+ * flags, seed, rng_stream and the order of operations are those of ng_gemm, but relu
+ * keeps NaN (ng_gemm's makes it 0): a block marked NaN stays visible.
  * workspace: 16-byte aligned, ng_mx_gemm_workspace_bytes() (0: may be NULL); with less
  * the call returns NG_MX_WORKSPACE and launches nothing. */
 #define NG_MX_WORKSPACE (-102)

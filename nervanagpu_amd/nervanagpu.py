@@ -760,6 +760,7 @@ class NervanaGPU(object):
         fp16 tensor (any order of its axes; the values of the block-scaled one are then
         taken as fp16).  Blocks run along k: A has axis 1, B has axis 0.
         C: fp16 or fp32, rows or columns contiguous; stochastic rounding as in dot.
+        relu keeps NaN, unlike dot's: a block that is marked NaN stays visible.
         """
         if type(A) is MXTensor:
             if type(B) is MXTensor and not A.fmt == B.fmt == "fp4":

@@ -43,3 +43,29 @@ def test_relu_below_a_dense_layer_keeps_what_is_not_a_number(ng):
     dx = layer.bprop(ng.array(rng.standard_normal((nout, N)).astype(np.float16))).get()
     bad = np.isnan(dx)
     assert bad[5, :32].all() and bad.sum() == 32
+
+
+@pytest.mark.parametrize("kinds", ["44", "4h", "h4", "8h", "h8"])
+@pytest.mark.parametrize("m,n,k", [(40, 24, 200), (35, 21, 200), (40, 1, 200), (33, 40, 2600), (70, 9, 2600)])
+@pytest.mark.parametrize("out,rounding", [(np.float16, 0), (np.float16, 10), (np.float32, 0)])
+def test_rectified_products_keep_what_is_not_a_number(ng, kinds, m, n, k, out, rounding):
+    """a row of A and a column of B whose block is NaN reach the result with relu as they do without; the rest is
+    the rectified product of small integers, which every store and its roundings hold exactly"""
+    rng = np.random.default_rng(m + n)
+    a = rng.integers(-2, 3, (m, k)).astype(np.float16)
+    b = (rng.integers(-2, 3, (k, n)) * (rng.random((k, n)) < 0.1)).astype(np.float16)
+    ref = np.maximum(a.astype(np.float64) @ b.astype(np.float64), 0)
+    assert ref.max() < 2048
+    ref[m // 2] = np.nan
+    a[m // 2, k - 1] = np.nan
+    if n > 1:
+        ref[:, n - 1] = np.nan
+        b[3, n - 1] = np.nan
+    side = {"h": lambda x, axis: ng.array(x), "4": lambda x, axis: ng.mx_array(x, "fp4", axis, rounding=0),
+            "8": lambda x, axis: ng.mx_array(x, "int8", axis, rounding=0)}
+    A, B = side[kinds[0]](a, 1), side[kinds[1]](b, 0)
+    for beta in (0.0, 1.0):
+        C = ng.ones((m, n), dtype=out)
+        C.rounding = rounding
+        ng.mx_dot(A, B, C, beta=beta, relu=True)
+        assert np.array_equal(C.get(), (ref + beta).astype(out), equal_nan=True)
