@@ -157,10 +157,11 @@ NG_DEV void mx_decode8(const unsigned (&in)[2], unsigned scale_byte, float (&v)[
 #pragma unroll
         for (int i = 0; i < 8; i++) v[i] = grid[i] * s;
     } else {
+        const float unit = s * 0.015625f;      // exact, subnormal units too, and so is a product with a code
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             const int q = (int)(in[i / 4] << (24 - 8 * (i & 3))) >> 24;
-            v[i] = (float)q * 0.015625f * s;   // 1/64 is exact, so is the product unless it leaves the fp32 range
+            v[i] = (float)q * unit;
         }
     }
 }

@@ -69,3 +69,71 @@ def test_rectified_products_keep_what_is_not_a_number(ng, kinds, m, n, k, out, r
         C.rounding = rounding
         ng.mx_dot(A, B, C, beta=beta, relu=True)
         assert np.array_equal(C.get(), (ref + beta).astype(out), equal_nan=True)
+
+
+EPS32, HALF16 = 2.0 ** -24, 2.0 ** -11
+
+
+def _close(got, ref, tol, what):
+    """within tol, and for fp16 half a unit of the result (2^-11 of its value, 2^-25 among the subnormal numbers); tol and
+    the reference are in 64 bits and both have the result's own magnitude, however small that is"""
+    if got.dtype == np.float16:
+        tol = tol * (1 + HALF16) + np.maximum(np.abs(ref) * HALF16, 2.0 ** -25)
+    else:
+        tol = tol + np.maximum(np.abs(ref) * EPS32, 2.0 ** -149)
+    off = np.abs(got.astype(np.float64) - ref)
+    worst = np.argmax(off - tol)
+    assert np.all(off <= tol), "%s: %g instead of %g, %g allowed" % (what, got.flat[worst], ref.flat[worst], tol.flat[worst])
+
+
+def _all_halves(lo, hi):
+    h = np.arange(65536, dtype=np.uint16).view(np.float16)
+    h = h[np.isfinite(h)]
+    h = np.sort(h[(h >= lo) & (h <= hi)])
+    return np.concatenate([h, np.zeros(-len(h) % 96, dtype=np.float16)]).reshape(-1, 96)
+
+
+def _checkpoints(top):
+    """values that 8-bit codes hold exactly: lines of one block, codes -127 .. 127 of every scale that reaches up to `top`"""
+    codes = np.concatenate([np.arange(-127, 128), [127]])
+    rows = [np.append(part[:-1], 127) * 2.0 ** e for e in range(int(np.log2(top)) - 6, -12, -1) for part in codes.reshape(-1, 32)]
+    return np.array(rows, dtype=np.float32)
+
+
+# Bounds in units of 2^-24 of the value.  fp16 operands: the tail Phi(-x) is a bell times a polynomial's quotient.  The quotient is off by
+# its fit (2.0e-6: 34 units), the argument t of its polynomial (3 units, which count 2.7-fold at most) and 6 steps of it (8); the bell by the
+# exponential (2) and by its argument's two roundings (z^2); three products: 55 + z^2 in all.  fp32 operands: erfc 16 ulp (32 units),
+# its argument's two roundings (2 z^2), two products.  The tail's complement adds one rounding of a value above 1/2.
+def _gelu_units(z, dtype):
+    return 56 + z * z if dtype == np.float16 else 35 + 2 * z * z
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_gelu_keeps_the_digits_of_its_left_tail(ng, dtype):
+    """every fp16 argument up to where the result vanishes, and for fp32 as far as the result is a normal number: the bound follows
+    the result itself"""
+    z = _all_halves(-6.5, 20) if dtype == np.float16 else np.linspace(-12.5, 12.5, 96 * 40, dtype=np.float32).reshape(-1, 96)
+    Y = ng.empty(z.shape, dtype=dtype)
+    ng.fprop_act("gelu", ng.array(z, dtype=dtype), Y)
+    zd = z.astype(np.float64)
+    ref = orc.ref_act("gelu", zd)
+    _close(Y.get(), ref, _gelu_units(zd, dtype) * EPS32 * np.abs(ref), "gelu")
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("error", [1.0, 1024.0])
+def test_gelu_slope_keeps_the_digits_of_its_left_tail(ng, dtype, error):
+    """Phi(z) + z phi(z): each of the two to its own digits (they cancel near z = -0.75 alone), then one sum and one product"""
+    z = _checkpoints(8.0)
+    q = ng.mx_array(z, "int8", rounding=0)
+    assert np.array_equal(q.get(), z)
+    G = ng.empty(z.shape, dtype=dtype)
+    ng.bprop_act("gelu", q, ng.array(np.full(z.shape, error, dtype=dtype), dtype=dtype), G)
+    zd = z.astype(np.float64)
+    parts = orc.ref_act("gelu", -np.abs(zd)) / np.where(zd == 0, -1, -np.abs(zd)) * (zd != 0) + 0.5 * (zd == 0) \
+        + np.abs(zd) * np.exp(-0.5 * zd * zd) / np.sqrt(2 * np.pi)
+    ref = error * orc.ref_act_slope("gelu", zd)
+    tol = EPS32 * (error * _gelu_units(zd, dtype) * parts + 3 * np.abs(ref))
+    # beyond |z| = 13 the tail and the density are subnormal numbers, off by up to a unit of 2^-149, which |z| and the error multiply
+    tol += error * (1 + np.abs(zd)) * 2.0 ** -149
+    _close(G.get(), ref, tol, "slope of gelu")
