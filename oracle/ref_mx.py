@@ -122,8 +122,8 @@ def ref_act_slope(op, z):
     if op == "relu":
         return np.where(np.isnan(z), np.nan, z > 0)
     if op == "tanh":
-        return 1.0 - np.tanh(z) ** 2
+        return 4.0 * _logistic(2.0 * z) * _logistic(-2.0 * z)      # 1 - tanh(z)^2 without its cancellation
     if op == "gelu":
         return 0.5 * _erfc(-z / math.sqrt(2.0)) + z * np.exp(-0.5 * z * z) / math.sqrt(2.0 * math.pi)
-    s = _logistic(z)
-    return s * (1.0 - s) if op == "sig" else s * (1.0 + z * (1.0 - s))
+    s, rest = _logistic(z), _logistic(-z)
+    return s * rest if op == "sig" else s * (1.0 + z * rest)

@@ -94,7 +94,7 @@ def _all_halves(lo, hi):
 
 
 def _checkpoints(top):
-    """values that 8-bit codes hold exactly: lines of one block, codes -127 .. 127 of every scale that reaches up to `top`"""
+    """values that 8-bit codes hold exactly: lines of one block, codes -127 .. 127 of every scale, to nearly twice `top`"""
     codes = np.concatenate([np.arange(-127, 128), [127]])
     rows = [np.append(part[:-1], 127) * 2.0 ** e for e in range(int(np.log2(top)) - 6, -12, -1) for part in codes.reshape(-1, 32)]
     return np.array(rows, dtype=np.float32)
@@ -137,3 +137,28 @@ def test_gelu_slope_keeps_the_digits_of_its_left_tail(ng, dtype, error):
     # beyond |z| = 13 the tail and the density are subnormal numbers, off by up to a unit of 2^-149, which |z| and the error multiply
     tol += error * (1 + np.abs(zd)) * 2.0 ** -149
     _close(G.get(), ref, tol, "slope of gelu")
+
+
+# Units of 2^-24 of the slope.  With t = e^-|z| (tanh: e^-2|z|) and r = 1 / (1 + t) the slopes are t r r and 4 t r r.  fp32 operands: exp
+# 3 ulp (6 units); of it r takes at most half, its sum and quotient 1 + 5, twice; two products: 26.  fp16 operands: exp and reciprocal 1 ulp
+# (2 units) and the two roundings of the exponent (2 units a unit of its argument, of which r's take at most half, twice): 12 + 4 |z|.
+def _saturated_units(op, z, dtype):
+    if dtype == np.float32:
+        return 26 + 0 * z
+    return 12 + 4 * np.abs(z) * (2 if op == "tanh" else 1)
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("op", ["sig", "tanh"])
+@pytest.mark.parametrize("error", [1.0, -1024.0])
+def test_slopes_of_saturated_functions(ng, dtype, op, error):
+    """sig' and tanh' fall like e^-|z| and e^-2|z| on both sides: the bound follows them"""
+    z = _checkpoints(16.0)
+    q = ng.mx_array(z, "int8", rounding=0)
+    assert np.array_equal(q.get(), z)
+    G = ng.empty(z.shape, dtype=dtype)
+    ng.bprop_act(op, q, ng.array(np.full(z.shape, error, dtype=dtype), dtype=dtype), G)
+    zd = z.astype(np.float64)
+    t = np.exp(-np.abs(zd) * (2 if op == "tanh" else 1))
+    ref = error * (4 if op == "tanh" else 1) * t / (1 + t) ** 2
+    _close(G.get(), ref, (_saturated_units(op, zd, dtype) + 1) * EPS32 * np.abs(ref), op)
