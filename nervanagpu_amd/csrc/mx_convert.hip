@@ -272,11 +272,13 @@ void mx_dequantize_across_kernel(const unsigned char* __restrict__ codes, const 
 // library's erfc alone kept the kernel from the memory's rate (backward gelu of 134M values: 275 us
 // with it).  fp32 takes the library's functions.
 //
-// 1 / (1 + e^-z); e^-z = inf gives 0
+// 1 / (1 + e^-z); where e^-z is infinite, below -88, the value is zero in fp16.  fp32 takes
+// e^z / (1 + e^z) on the left, whose tail goes on to -103.
 template <bool FAST> NG_DEV float act_logistic(float z)
 {
     if (FAST) return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f));
-    return 1.0f / (1.0f + expf(-z));
+    const float t = expf(-__builtin_fabsf(z)), r = 1.0f / (1.0f + t);
+    return z < 0.0f ? t * r : r;
 }
 // logistic(z) logistic(-z) as t / (1 + t)^2 with t = e^-|z|: one less the other factor would
 // keep none of its digits where the function saturates

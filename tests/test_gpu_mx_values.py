@@ -162,3 +162,24 @@ def test_slopes_of_saturated_functions(ng, dtype, op, error):
     t = np.exp(-np.abs(zd) * (2 if op == "tanh" else 1))
     ref = error * (4 if op == "tanh" else 1) * t / (1 + t) ** 2
     _close(G.get(), ref, (_saturated_units(op, zd, dtype) + 1) * EPS32 * np.abs(ref), op)
+
+
+@pytest.mark.parametrize("op", ["sig", "silu"])
+def test_logistic_functions_keep_their_left_tail(ng, op):
+    """fp32, as far as the value is a normal number (e^-87): e^z (1 + e^z)^-1 needs no e^-z, which leaves the range of fp32 there.
+    exp 3 ulp (6 units), a sum and a quotient (6 and at most half of exp's), two products; what underflows on the way is off by 2^-149,
+    times z for silu"""
+    z = np.linspace(-103.0, 30.0, 96 * 40, dtype=np.float32).reshape(-1, 96)
+    Y = ng.empty(z.shape, dtype=np.float32)
+    ng.fprop_act(op, ng.array(z, dtype=np.float32), Y)
+    zd = z.astype(np.float64)
+    ref = orc.ref_act(op, zd)
+    tol = 18 * EPS32 * np.abs(ref) + 3 * 2.0 ** -149 * (np.abs(zd) if op == "silu" else 1)
+    _close(Y.get(), ref, tol, op)
+    q = ng.mx_array(np.tile(np.arange(-103, -71, dtype=np.float32), (2, 1)), "int8", rounding=0)
+    if op == "silu":
+        G = ng.ones((2, 32), dtype=np.float32)
+        ng.bprop_act(op, q, G, G)
+        zq = q.get().astype(np.float64)
+        ref = orc.ref_act_slope(op, zq)
+        _close(G.get(), ref, 18 * EPS32 * np.abs(ref) + 3 * 2.0 ** -149 * np.abs(zq), "slope of silu")
