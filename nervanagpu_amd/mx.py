@@ -50,6 +50,7 @@ class MXTensor(object):
             raise ValueError("bad axis for an MXTensor")
         self.shape = tuple(int(extent) for extent in shape)
         assert len(self.shape) == 2 and min(self.shape) >= 0, "block-scaled tensors are matrices"
+        assert max(self.shape) < 2 ** 31, "extents of block-scaled tensors stay below 2^31"
         self.backend, self.fmt, self.axis = backend, fmt, axis
         self.rounding, self.name = rounding, name
         self.size = self.shape[0] * self.shape[1]

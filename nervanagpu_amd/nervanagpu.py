@@ -703,6 +703,8 @@ class NervanaGPU(object):
         assert len(shape) == 2 and not A.take_array, "%s must be a 2-D tensor" % what
         inner, outer = strides[axis], strides[1 - axis]
         depth, lines = shape[axis], shape[1 - axis]
+        # the C interface takes extents as ints
+        assert depth < 2 ** 31 and lines < 2 ** 31, "%s has an extent of 2^31 or more" % what
         if inner == 1:
             if outer >= depth:
                 return outer, 1
