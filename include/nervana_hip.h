@@ -250,7 +250,12 @@ enum ng_mx_format { NG_MX_NONE = 0, NG_MX_FP4 = 1, NG_MX_INT8 = 2 };
  * A[i * lda + line] (along = 0).  Rounding is to the nearest, ties to the even
  * code; with NG_FLAG_SR each value takes one of its two neighbours with the
  * probability that makes it right on average (element line * depth + i of the stream
- * (seed, rng_stream)).  A block that holds an infinity or a NaN becomes NaN. */
+ * (seed, rng_stream)).  The scale follows from the block's largest magnitude m, by
+ * floor(log2 m), so that a code may end below m: nearest fp4 takes what lies above 6
+ * as 6; int8 takes what lies above 127/64 (at most the top 1/128 of m's power of two) as
+ * 127/64 in either mode, so there, and only there, its stochastic rounding is off on average,
+ * by less than 1/64 of the scale.  Stochastic fp4 takes one power more where m is above 6: no
+ * value of it saturates.  A block that holds an infinity or a NaN becomes NaN. */
 int ng_mx_quantize(int format, int dtype, const void* A, long lda, int along, int lines, int depth,
                    void* codes, void* scales, unsigned flags, unsigned seed, unsigned rng_stream, void* stream);
 /* out (dtype NG_F16 or NG_F32, laid out like A above) = the values, rounded to the

@@ -40,7 +40,8 @@ class MXTensor(object):
     codes, scales: uint8 GPUTensors to use instead of new ones, of (lines,
            code_pitch) and (lines, scale_pitch); codes beyond the last value of a
            line must be zero
-    rounding: non-zero: mx_quantize rounds stochastically into this tensor
+    rounding: non-zero: mx_quantize rounds stochastically into this tensor (right on
+           average; int8 values above 127/64 of their block's power of two saturate)
     """
 
     def __init__(self, backend, shape, fmt="fp4", axis=1, codes=None, scales=None, rounding=0, name=None):

@@ -722,7 +722,9 @@ class NervanaGPU(object):
         """out = A in blocks of 32 values that share a power of two.  A: fp16 or fp32
         matrix with one contiguous dimension.  Rounds to the nearest code (ties to
         even), or stochastically if out.rounding is set: then every value is right on
-        average.  A block with an infinity or a NaN becomes NaN.  Returns out."""
+        average, but for int8 values above the last code (127/64 of the block's power of
+        two, at most 128/64), which become 127/64 in either mode.  A block with an
+        infinity or a NaN becomes NaN.  Returns out."""
         assert type(out) is MXTensor and A.shape == out.shape
         if A.dtype.type not in _FLOATS:
             raise TypeError("Only floating point tensors can be quantized.")

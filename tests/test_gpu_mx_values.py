@@ -183,3 +183,23 @@ def test_logistic_functions_keep_their_left_tail(ng, op):
         zq = q.get().astype(np.float64)
         ref = orc.ref_act_slope(op, zq)
         _close(G.get(), ref, 18 * EPS32 * np.abs(ref) + 3 * 2.0 ** -149 * np.abs(zq), "slope of silu")
+
+
+@pytest.mark.parametrize("axis", [0, 1])
+@pytest.mark.parametrize("top", [127.0, 127.5, 127.984375])
+def test_stochastic_int8_is_right_on_average_up_to_its_last_code(ng, axis, top):
+    """units of the block are 1 here (its largest value lies in 64 .. 128).  Up to 127 units the mean of n draws is right: between
+    neighbours 1 apart its variance is at most 1 / 4n, 6 sigma are 3 / sqrt(n), and the 16 bits of the definition add 2^-16.  Above there
+    is no code: such values become 127 in every draw, stochastic or not"""
+    n = 4096
+    row = np.zeros(32, dtype=np.float32)
+    row[:9] = [top, 126.75, -126.25, 100.5, -64.1, 12.3, 0.4, -0.03, -top]
+    x = np.tile(row, (n, 1)) if axis == 1 else np.tile(row[:, None], (1, n))
+    q = ng.mx_empty(x.shape, "int8", axis, rounding=1)
+    got = ng.mx_quantize(ng.array(x, dtype=np.float32), q).get().astype(np.float64)
+    got = got if axis == 1 else got.T
+    below = np.abs(row) <= 127
+    assert np.all(np.abs(got.mean(axis=0) - row)[below] <= 3 / np.sqrt(n) + 2.0 ** -16)
+    assert np.all(got[:, ~below] == np.sign(row[~below]) * 127)
+    nearest = ng.mx_quantize(ng.array(x, dtype=np.float32), ng.mx_empty(x.shape, "int8", axis, rounding=0)).get()
+    assert np.array_equal((nearest if axis == 1 else nearest.T)[0][~below], np.sign(row[~below]) * 127)

@@ -18,6 +18,6 @@ def _emulate(name, expr, cus="8"):
     assert " passed" in tail and "failed" not in tail, tail
 
 
-@pytest.mark.parametrize("expr", ["relu", "rectified", "gelu", "saturated", "logistic"])
+@pytest.mark.parametrize("expr", ["relu", "rectified", "gelu", "saturated", "logistic", "int8"])
 def test_values_on_the_emulator(expr):
     _emulate("test_gpu_mx_values.py", expr)
