@@ -127,8 +127,17 @@ void vmem_wait(int outstanding)
     while ((int)q.size() > outstanding) { apply(q.front()); q.pop_front(); }
 }
 
-void launch(dim3 grid, dim3 block, const std::function<void()>& body, const char* name)
+// instead of running anything: a line per launch, its grid, the kernel and the function that launches it
+static bool g_dry = false;
+static std::string g_launches;
+
+void launch(dim3 grid, dim3 block, const std::function<void()>& body, const char* name, const char* kernel)
 {
+    if (g_dry) {
+        g_launches += std::to_string(grid.x) + "," + std::to_string(grid.y) + "," + std::to_string(grid.z) + " " +
+                      std::to_string(block.x) + " " + (kernel ? kernel : "") + " " + (name ? name : "") + "\n";
+        return;
+    }
     const int nthreads = (int)(block.x * block.y * block.z);
     const int nwaves = (nthreads + 63) / 64;
     g_grid = grid; g_block = block;
@@ -403,6 +412,9 @@ int ng_launch(void* function, const unsigned grid[3], const unsigned block[3], u
 
 // controls of the emulation
 void emu_set_cus(int cus) { emu::g_cus = cus; }
+// dry: launches are listed and not run; emu_launches returns the list, emu_set_dry starts a new one
+void emu_set_dry(int dry) { emu::g_dry = dry != 0; emu::g_launches.clear(); }
+const char* emu_launches(void) { return emu::g_launches.c_str(); }
 void emu_set_late_loads(int late) { emu::g_late_loads = late != 0; }
 void emu_set_shuffle(unsigned seed) { emu::g_shuffle_seed = seed; }
 void emu_register_buffer(const void* p, size_t bytes) { g_buffers[(uintptr_t)p] = bytes; }
