@@ -1142,7 +1142,8 @@ template <> struct StoreBits<float> {
 
 // alpha -> relu -> + beta*C -> round -> store
 // (order of kernels/sass/hgemm_common_128x128.sass:183-264 in the reference)
-template <typename T>
+// RELU_KEEPS_NAN: relu of NaN is NaN, else 0 as the maximum of the two
+template <typename T, bool RELU_KEEPS_NAN = false>
 struct ScaleStoreEpilogue {
     typedef typename StoreBits<T>::bits_t bits_t;
     T*       C;
@@ -1188,10 +1189,15 @@ struct ScaleStoreEpilogue {
         for (int e = 0; e < 8; e++) out[e] = (StoreBits<T>::widen(mk[e]) > 0.0f) ? out[e] : (bits_t)0;
     }
 
+    static __device__ __forceinline__ float rectified(float v)
+    {
+        if constexpr (RELU_KEEPS_NAN) return v <= 0.0f ? 0.0f : v;
+        else                          return fmaxf(v, 0.0f);
+    }
     __device__ __forceinline__ float scale(float acc) const
     {
         float v = acc * alpha;
-        return relu ? fmaxf(v, 0.0f) : v;
+        return relu ? rectified(v) : v;
     }
     __device__ __forceinline__ unsigned rng_index(int i, int j, int z) const
     {
@@ -1214,7 +1220,7 @@ struct ScaleStoreEpilogue {
         bits_t out[8];
         if (relu) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) out[e] = StoreBits<T>::round(fmaxf(acc[e] * alpha, 0.0f), 0, 0, 0, 0);
+            for (int e = 0; e < 8; e++) out[e] = StoreBits<T>::round(rectified(acc[e] * alpha), 0, 0, 0, 0);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; e++) out[e] = StoreBits<T>::round(acc[e] * alpha, 0, 0, 0, 0);
@@ -1267,7 +1273,7 @@ struct ScaleStoreEpilogue {
             bits_t out[8];
             if (relu) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) out[e] = StoreBits<T>::round(fmaxf(acc[e] * alpha, 0.0f), 0, 0, 0, 0);
+                for (int e = 0; e < 8; e++) out[e] = StoreBits<T>::round(rectified(acc[e] * alpha), 0, 0, 0, 0);
             } else {
 #pragma unroll
                 for (int e = 0; e < 8; e++) out[e] = StoreBits<T>::round(acc[e] * alpha, 0, 0, 0, 0);

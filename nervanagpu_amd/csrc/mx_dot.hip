@@ -214,10 +214,9 @@ static int launch_product(const MxArgs& g, const MxSide& a, const MxSide& b)
     s.tiles_n = ceil_div(g.n, p.bn);
     const int tiles = s.tiles_m * s.tiles_n;
     const dim3 grid(grid_tiles(tiles, s.splits), grid_slices(tiles, s.splits), 1);
-    const MxStoreEpilogue<T> epi{{(T*)g.C, 0, g.ldc, g.m, g.n, 1.0f, g.beta, 0u,
+    const MxStoreEpilogue<T> epi{{(T*)g.C, 0, g.ldc, g.m, g.n, g.alpha, g.beta, (g.flags & NG_FLAG_RELU) ? 1u : 0u,
                                   mx_sr_bits(g.flags, g.c_dtype), g.seed, g.rng_stream,
-                                  (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u},
-                                 g.alpha, (g.flags & NG_FLAG_RELU) ? 1u : 0u};
+                                  (((uintptr_t)g.C & 15) == 0 && g.ldc % 8 == 0 && g.n % 8 == 0) ? 1u : 0u}};
     if constexpr ((FA == NG_MX_FP4) != (FB == NG_MX_FP4)) {
         if (p.skinny) return launch_skinny<FA == NG_MX_FP4>(g, p.skinny, FA == NG_MX_FP4 ? a : b, FA == NG_MX_FP4 ? b : a, epi);
     }

@@ -759,42 +759,19 @@ void mxmix_kernel(MxSide x, MxSide d, Epi epi, CoreShape s)
     EpilogueBands<TM, TN, WTN, EPITCH, 0>::run(acc, stage, lane, m0 + wm * TM * 32, n0 + wn * WTN, 0, split, epi);
 }
 
-// The stores of a product: those of ScaleStoreEpilogue, except that
-//  - relu keeps NaN, the mark of a block with an infinity or a NaN (fmaxf would make it 0): the
-//    base gets values that are scaled and rectified already, its own factor is 1 and its relu off;
-//  - 8 neighbouring values of a row that is not 16-byte aligned (an odd row length) still go out
-//    in wide stores, which the hardware takes at any alignment, instead of one by one
-//    (4001x5003 fp32 outputs of fp16 by int8, k = 64: 64 us one by one, 28 us so).  Of
-//    PartialEpilogue likewise.
+// The stores of a product: those of ScaleStoreEpilogue, whose relu keeps NaN here (the mark of a
+// block with an infinity or a NaN shows in a rectified product), and PartialEpilogue, except that 8
+// neighbouring values of a row that is not 16-byte aligned (an odd row length) still go out
+// in wide stores, which the hardware takes at any alignment, instead of one by one
+// (4001x5003 fp32 outputs of fp16 by int8, k = 64: 64 us one by one, 28 us so).
 template <typename T>
-struct MxStoreEpilogue : ScaleStoreEpilogue<T> {
-    typedef ScaleStoreEpilogue<T> Base;
+struct MxStoreEpilogue : ScaleStoreEpilogue<T, true> {
+    typedef ScaleStoreEpilogue<T, true> Base;
     typedef typename Base::bits_t bits_t;
-    float factor;
-    unsigned rectify;
-    __device__ __forceinline__ float value(float acc) const
-    {
-        const float v = acc * factor;
-        return rectify && v <= 0.0f ? 0.0f : v;
-    }
-    __device__ __forceinline__ void values(const float (&acc)[8], float (&v)[8]) const
-    {
-#pragma unroll
-        for (int e = 0; e < 8; e++) v[e] = value(acc[e]);
-    }
-    __device__ __forceinline__ void apply(int i, int j, int z, float acc) const { Base::apply(i, j, z, value(acc)); }
-    __device__ __forceinline__ void store8_buffer(BufferRsrc rsrc, int i, int j0, const float (&acc)[8]) const
-    {
-        float v[8];
-        values(acc, v);
-        Base::store8_buffer(rsrc, i, j0, v);
-    }
     __device__ __forceinline__ void store8(int i, int j0, int z, int split, const float (&acc)[8]) const
     {
-        float v[8];
-        values(acc, v);
         if (this->vec || i >= this->m || j0 + 8 > this->n) {
-            Base::store8(i, j0, z, split, v);
+            Base::store8(i, j0, z, split, acc);
             return;
         }
         bits_t* p = reinterpret_cast<bits_t*>(this->C + (long)i * this->ldc + j0);
@@ -802,8 +779,9 @@ struct MxStoreEpilogue : ScaleStoreEpilogue<T> {
         if (this->beta != 0.0f) __builtin_memcpy(out, p, sizeof(out));
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            if (this->beta != 0.0f) v[e] += this->beta * StoreBits<T>::widen(out[e]);
-            out[e] = StoreBits<T>::round(v[e], this->sr_bits, this->seed, this->stream, this->rng_index(i, j0 + e, z));
+            float v = this->scale(acc[e]);
+            if (this->beta != 0.0f) v += this->beta * StoreBits<T>::widen(out[e]);
+            out[e] = StoreBits<T>::round(v, this->sr_bits, this->seed, this->stream, this->rng_index(i, j0 + e, z));
         }
         __builtin_memcpy(p, out, sizeof(out));
     }

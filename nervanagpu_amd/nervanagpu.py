@@ -704,7 +704,7 @@ class NervanaGPU(object):
         inner, outer = strides[axis], strides[1 - axis]
         depth, lines = shape[axis], shape[1 - axis]
         # the C interface takes extents as ints
-        assert depth < 2 ** 31 and lines < 2 ** 31, "%s has an extent of 2^31 or more" % what
+        assert (depth | lines) < 2 ** 31, "%s has an extent of 2^31 or more" % what
         if inner == 1:
             if outer >= depth:
                 return outer, 1
