@@ -255,11 +255,14 @@ enum ng_mx_format { NG_MX_NONE = 0, NG_MX_FP4 = 1, NG_MX_INT8 = 2 };
  * as 6; int8 takes what lies above 127/64 (at most the top 1/128 of m's power of two) as
  * 127/64 in either mode, so there, and only there, its stochastic rounding is off on average,
  * by less than 1/64 of the scale.  Stochastic fp4 takes one power more where m is above 6: no
- * value of it saturates.  A block that holds an infinity or a NaN becomes NaN. */
+ * value of it saturates.  A block that holds an infinity or a NaN becomes NaN.
+ * Limits: extents below 2^31 - 256; along = 1: below 2^34 values with every line's last block
+ * counted whole; along = 0: depth of at most 65535 * 128. */
 int ng_mx_quantize(int format, int dtype, const void* A, long lda, int along, int lines, int depth,
                    void* codes, void* scales, unsigned flags, unsigned seed, unsigned rng_stream, void* stream);
 /* out (dtype NG_F16 or NG_F32, laid out like A above) = the values, rounded to the
- * nearest where fp16 does not hold them exactly */
+ * nearest where fp16 does not hold them exactly.  Limits as above, but along = 0: depth of at
+ * most 65535 * 64. */
 int ng_mx_dequantize(int format, const void* codes, const void* scales, int lines, int depth,
                      int dtype, void* out, long ldo, int along, void* stream);
 
@@ -268,8 +271,9 @@ int ng_mx_dequantize(int format, const void* codes, const void* scales, int line
  *   ng_act_fprop  O = f(I); codes and scales, unless NULL, receive I; O may be I
  *   ng_act_bprop  gradI = E * f'(the values of the checkpoint); gradI may be E
  * E, O and gradI have the dtype (NG_F16 or NG_F32) of I; ldi, ldo, lde, ldg are row
- * pitches in elements.  NaN stays NaN, under relu too: a block of the checkpoint that holds
- * one infinity or NaN makes its 32 values of gradI NaN. */
+ * pitches in elements.  Results are rounded to the nearest.  NaN stays NaN, under relu
+ * too: a block of the checkpoint that holds one infinity or NaN makes its 32 values of
+ * gradI NaN. */
 enum ng_act { NG_ACT_RELU = 0, NG_ACT_SIG = 1, NG_ACT_TANH = 2, NG_ACT_SILU = 3, NG_ACT_GELU = 4 };
 int ng_act_fprop(int act, int dtype, int rows, int cols, const void* I, long ldi, void* O, long ldo,
                  void* codes, void* scales, void* stream);
@@ -279,7 +283,8 @@ int ng_act_bprop(int act, int dtype, int rows, int cols, const void* codes, cons
 /* C = round(beta*C + relu(alpha * A.B)) where A (m, k) and B (k, n) are block
  * scaled along k, or one of them is and the other is a dense fp16 matrix:
  *   fp4 . fp4, fp4 . fp16, fp16 . fp4, int8 . fp16, fp16 . int8.
- * C is fp16 or fp32 (c_dtype), row-major with row pitch ldc; fp32 accumulation.
+ * C is fp16 or fp32 (c_dtype), row-major with row pitch ldc, and overlaps neither operand;
+ * fp32 accumulation.
  * Block-scaled operand: format, codes, scales; lines are the rows of A / the columns
  * of B.  Beside a dense operand its values are first rounded to fp16, which changes
  * nothing if they came from fp16.

@@ -270,7 +270,8 @@ def main(argv=None):
                          "the layer below them (same results, one elementwise pass per such pair saved; not in "
                          "the reference)")
     ap.add_argument("--fc-mx4", action="store_true",
-                    help="fp16 networks: dense layers multiply 4-bit block-scaled copies of weights, inputs and errors")
+                    help="fp16 networks: dense layers multiply 4-bit block-scaled copies of weights, inputs and errors (slower "
+                         "at these networks' minibatches: the copies of the weights cost more than their products save)")
     ap.add_argument("--fc-save8", action="store_true",
                     help="fp16 networks: dense layers keep their input for the backward pass in 8 bits")
     args = ap.parse_args(argv)

@@ -1,10 +1,15 @@
 // Conversions between dense and block-scaled matrices, and the activation
 // functions that keep an 8-bit checkpoint of their input.  All of them read each value once
-// and write it once.  fp16 of 16384x8192, against 4.9 TB/s of a large copy:
-//   backward gelu from the checkpoint   115 us, 675 MB, 5.9 TB/s: memory
-//   fp4 to fp16                          61 us, 340 MB, 5.5 TB/s: memory
-//   fp16 to fp4, stochastic             118 us, 340 MB, 2.9 TB/s: the vector unit (two 32-bit
+// and write it once.  fp16 of 16384x8192, calls back to back, against 4.9 TB/s of a large copy:
+//   backward gelu from the checkpoint   116 us, 675 MB, 5.8 TB/s: memory, and the vector unit close behind
+//   forward silu with checkpoint        110 us, 675 MB, 6.1 TB/s: memory (gelu 122, tanh 133: the library's)
+//   fp16 to fp4, nearest                 58 us, 340 MB, 5.9 TB/s: memory
+//   ... stochastic                       91 us, 340 MB, 3.7 TB/s: the vector unit (two 32-bit
 //                                        products of the random word a pair of values, 10 operations a value)
+//   fp4 to fp16                          67 us, 340 MB, 5.0 TB/s: memory
+//   fp16 to int8 and back                70 (stochastic 80) and 69 us, 407 MB: memory
+//   across the rows                      fp4 171 (186) and 109 us, int8 187 (192) and 120 us: a workgroup's rows are
+//                                        128 bytes each, the codes of its lines 64 to 128
 // and at 4096x128 the launch: 2.3 to 3.9 us a kernel.
 #include "mx_format.h"
 

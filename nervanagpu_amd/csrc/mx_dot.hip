@@ -130,7 +130,7 @@ static MxPlan choose_plan(int m, int n, int k, const ng_mx_operand& A, const ng_
     } else if (tiles(128, 128) <= cus / 2 && tiles(128, 128) * std::max(1, ceil_div(k, 64) / least) < cus) {
         // a few workgroups wait out each tile's latency: four times as many where slices of the contraction do not
         // make up for them (512^3 7.5 us, 11.0 on 128x128 tiles; 600x900 outputs of k = 8000 66 us, 32 on 128x128 in slices;
-        // 4096x48 of k = 4096 14.7 and 15.5)
+        // 4096x48 of k = 4096 14.9 and 14.8)
         p.bm = p.bn = 64;
     }
     const int out_tiles = (int)std::min<long>(tiles(p.bm, p.bn), 1 << 30);

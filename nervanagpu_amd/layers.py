@@ -258,7 +258,8 @@ class FullLayer(Layer):
     mx4     y = W x and dx = W^T e multiply 4-bit block-scaled copies of W, x and e
             (blocks along the contraction of each product, made in every step; they
             round stochastically if the backend does).  The weights themselves and
-            their gradient stay as they are.
+            their gradient stay as they are.  Pays from minibatches of about a thousand
+            on (9216 -> 4096: a step of 4096 images 903 -> 659 us, of 128 108 -> 154).
     save8   the input is kept for the backward pass in 8 bits (saved_in): the weight
             gradient, and with relu_below the rectifier derivative of the layer
             below, are computed from what those stand for: NaN for the 32 values of a

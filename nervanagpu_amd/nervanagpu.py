@@ -736,7 +736,8 @@ class NervanaGPU(object):
         return out
 
     def mx_dequantize(self, A, out):
-        """out (fp16 or fp32) = the values of the block-scaled A; returns out"""
+        """out (fp16 or fp32) = the values of the block-scaled A, rounded to the nearest
+        whatever out.rounding says; returns out"""
         assert type(A) is MXTensor and A.shape == out.shape
         if out.dtype.type not in _FLOATS:
             raise TypeError("Only floating point tensors can be dequantized into.")
@@ -762,8 +763,9 @@ class NervanaGPU(object):
 
         A (m, k), B (k, n): both fp4, or one of them fp4 or int8 and the other a dense
         fp16 tensor (any order of its axes; the values of the block-scaled one are then
-        taken as fp16).  Blocks run along k: A has axis 1, B has axis 0.
-        C: fp16 or fp32, rows or columns contiguous; stochastic rounding as in dot.
+        taken as fp16: exact if they came from fp16, else far ones overflow or vanish).  Blocks run along k: A has axis 1, B has axis 0.
+        C: fp16 or fp32, rows or columns contiguous, on memory of its own; stochastic
+        rounding as in dot.
         relu keeps NaN, unlike dot's: a block that is marked NaN stays visible.
         """
         if type(A) is MXTensor:
@@ -847,7 +849,8 @@ class NervanaGPU(object):
         nearest, in one pass.
 
         op: "relu", "sig", "tanh", "silu" (x sig(x)) or "gelu" (x times the normal
-        distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous; O may be I
+        distribution function of x); I, O: fp16 or fp32 matrices, rows contiguous; O may
+        be I.  Stored rounded to the nearest, whatever O.rounding says.
         """
         code, dtype, rows, cols, codes, scales, (ldi, ldo) = self._act_operands(op, (I, O), saved)
         if I.size:
