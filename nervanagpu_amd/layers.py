@@ -314,6 +314,7 @@ class FullLayer(Layer):
         return self.fprop_out
 
     def bprop(self, bprop_in):
+        assert self.save8 or not self.relu_below, "relu_below of a dense layer needs save8"
         err = self.bprop_relu(bprop_in)
         if self.mx4:
             self.lib.mx_dot(self._mx_copy("W^T", self.weights, 0).T, self._mx_copy("e", err, 0), self.bprop_out)

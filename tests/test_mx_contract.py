@@ -23,3 +23,13 @@ def test_extents_that_do_not_fit_an_int_are_refused(calls, far):  # noqa: F811
         with pytest.raises(AssertionError, match="2\\^31"):
             ng.mx_dot(A, B, C)
     assert not calls
+
+
+def test_rectifier_below_a_layer_without_saved_input_is_refused():
+    """relu_below reads the saved input: without one the derivative of the layer below would be left out unseen"""
+    import numpy as np
+    from nervanagpu_amd.layers import FullLayer
+    layer = FullLayer(NervanaGPU(), np.float16, 32, 64, 16)
+    layer.relu_below = layer.relu_done_above = True
+    with pytest.raises(AssertionError, match="save8"):
+        layer.bprop(None)
