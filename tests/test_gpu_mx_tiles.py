@@ -78,3 +78,44 @@ def test_large_tiles_on_few_units(ng, kinds, m, n, k, kernel, slices, cus):
     if "emulation" in _lib.device_name() and os.environ.get("EMU_CUS") != str(cus):
         pytest.skip("for %d CUs" % cus)
     check(ng, kinds, m, n, k, outs=(np.float16,) if m > 257 else (np.float32,))
+
+
+def test_codes_beyond_32_bits_of_offset(ng):
+    """a matrix of 65600 lines of 131072 values: 4.3 GB of 4-bit codes, 8.6 GB of 8-bit ones, 17 GB of fp16.  The lines checked are the
+    first, those around 2^31 and 2^32 bytes, and the last; the others hold what the memory held (a line's products are its own)"""
+    import oracle as orc
+    from nervanagpu_amd import _lib
+    if "emulation" in _lib.device_name():
+        pytest.skip("needs 30 GB")
+    lines, depth = 65600, 131072
+    rng = np.random.default_rng(30)
+    big = ng.empty((lines, depth))
+    checked = [0, 8191, 8192, 16384, 32767, 32768, 65535, 65536, lines - 1]
+    x = (rng.standard_normal((len(checked), depth)) * np.exp2(rng.integers(-3, 4, (len(checked), 1)))).astype(np.float16)
+    for r, row in zip(checked, x):
+        _lib.memcpy_htod(big.ptr + 2 * r * depth, row)
+    dense = rng.standard_normal((depth, 40)).astype(np.float16)
+    back = np.empty(depth, dtype=np.float16)
+    for fmt in ("fp4", "int8"):
+        q = ng.mx_quantize(big, ng.mx_empty((lines, depth), fmt, rounding=0))
+        _, _, v = orc.ref_mx_round(x, fmt)
+        for count in (1, 16, 40) if fmt == "fp4" else (40,):
+            C = ng.empty((lines, count), dtype=np.float32)
+            ng.mx_dot(q, ng.array(dense[:, :count]), C)
+            _check_product(C.get()[checked], v, dense[:, :count].astype(np.float64), "%s by %d" % (fmt, count))
+        if fmt == "fp4":
+            few = ng.mx_array(dense, axis=0, rounding=0)
+            ng.mx_dot(q, few, C)
+            _check_product(C.get()[checked], v, few.get().astype(np.float64), "fp4 by fp4")
+        ng.mx_dequantize(q, big)
+        for r, row in zip(checked, v):
+            _lib.memcpy_dtoh(back, big.ptr + 2 * r * depth)
+            assert np.array_equal(back, row.astype(np.float16)), r
+        for r, row in zip(checked, x):
+            _lib.memcpy_htod(big.ptr + 2 * r * depth, row)
+    # in place, with a checkpoint that lies as far
+    ng.fprop_act("relu", big, big, saved=q)
+    ng.bprop_act("relu", q, big, big)
+    for r, row, value in zip(checked, x, v):
+        _lib.memcpy_dtoh(back, big.ptr + 2 * r * depth)
+        assert np.array_equal(back, np.where(value > 0, np.maximum(row, 0), 0)), r
