@@ -8,8 +8,8 @@
 //                                        products of the random word a pair of values, 10 operations a value)
 //   fp4 to fp16                          67 us, 340 MB, 5.0 TB/s: memory
 //   fp16 to int8 and back                70 (stochastic 80) and 69 us, 407 MB: memory
-//   across the rows                      fp4 171 (186) and 109 us, int8 187 (192) and 120 us: a workgroup's rows are
-//                                        128 bytes each, the codes of its lines 64 to 128
+//   across the rows                      fp4 171 (186) and 109 us, int8 187 (192) and 120 us (pieces of 128 bytes
+//                                        of a row, 64 to 128 of a line's codes)
 // and at 4096x128 the launch: 2.3 to 3.9 us a kernel.
 #include "mx_format.h"
 

@@ -763,10 +763,11 @@ class NervanaGPU(object):
 
         A (m, k), B (k, n): both fp4, or one of them fp4 or int8 and the other a dense
         fp16 tensor (any order of its axes; the values of the block-scaled one are then
-        taken as fp16: exact if they came from fp16, else far ones overflow or vanish).  Blocks run along k: A has axis 1, B has axis 0.
+        taken as fp16: exact if they came from fp16, else far ones overflow or vanish).
+        Blocks run along k: A has axis 1, B has axis 0.
         C: fp16 or fp32, rows or columns contiguous, on memory of its own; stochastic
-        rounding as in dot.
-        relu keeps NaN, unlike dot's: a block that is marked NaN stays visible.
+        rounding as in dot.  relu keeps NaN, unlike dot's: a block that is marked NaN
+        stays visible.
         """
         if type(A) is MXTensor:
             if type(B) is MXTensor and not A.fmt == B.fmt == "fp4":
